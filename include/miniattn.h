@@ -296,6 +296,106 @@ typedef struct MiniAttnLinearParams {
 int miniattn_linear(const MiniAttnLinearParams* p, void* stream);
 
 /*
+ * Attention over a cache (no counterpart in the reference, whose sequences of a batch are equally long and whole): K and V in
+ * pages that a block table names, sequences of different lengths in one call, a sliding window with sinks, a prefix that all
+ * sequences share.
+ *
+ * With seq_lens, sequence b holds seq_lens[b] tokens, its new ones (the rows of q) among them and last: query token i of
+ * n sits at position seq_lens[b] - n + i.  Without, it sits at diag + i and there are Nk keys.  It sees the keys at positions
+ * up to its own, with window > 0 only those at most window - 1 before it and the first `sinks` ones.  Rows that see no key
+ * (a length of 0, the front of a padded sequence) come out 0, their lse -inf.
+ *
+ * block_table: key j of sequence b lies in page block_table[b * table_stride + j / page_size], token j % page_size of it;
+ * k and v are [n_pages, page_size, Hkv, D] with any (page, head, token) strides.  Entries whose keys no row sees are not
+ * read, nor are those keys.  page_size 0: no pages, k and v are [B, Hkv, Nk, D], strides (batch, head, token).
+ *
+ * cu_q: the rows of sequence b are cu_q[b] .. cu_q[b + 1] - 1 of q, total_q rows in all; rows behind the last sequence's are
+ * left as they are.  Null: Nq rows each.
+ *
+ * shared_len: the first shared_len tokens of all sequences are the same, in the pages that sequence 0 names; their keys are
+ * read once for all.  A multiple of page_size; not with a window.
+ *
+ * A length, row number or page outside the call's tensors sets bit 7 of the status word; nothing outside them is read or
+ * written, and the sequence's results are undefined, the others' are not.
+ *
+ * Lengths, rows and pages are read on the device: a captured launch serves every length the block table has room for.
+ */
+typedef struct MiniAttnCacheParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void*       o;
+  float*      lse;        /* optional, fp32 ln(sum exp), the token's stride is 1       */
+  int32_t*    status;     /* as in MiniAttnFwdParams                                   */
+  const int32_t* block_table; /* [B, table_width]; null without pages                  */
+  const int32_t* seq_lens;    /* [B]; null without pages                               */
+  const int32_t* cu_q;        /* [B + 1] or null                                       */
+  int64_t q_stride[3];    /* (sequence, head, token); the first is not used with cu_q  */
+  int64_t k_stride[3];    /* (page or batch, head, token)                              */
+  int64_t v_stride[3];
+  int64_t o_stride[3];    /* as q_stride                                               */
+  int64_t lse_stride[2];  /* (sequence, head)                                          */
+  int64_t table_stride;
+  int64_t diag;           /* without pages                                         */
+  int32_t B, Hq, Hkv, D;
+  int32_t Nq;             /* rows of each sequence; with cu_q the most that one has,   */
+                          /* by which the kernel is chosen (0: not known)              */
+  int32_t total_q;        /* with cu_q: rows of q                                      */
+  int32_t Nk;             /* without pages                                         */
+  int32_t page_size;      /* 16, 32, 64, ... 1024; 0: no pages                     */
+  int32_t n_pages, table_width;
+  int32_t window;         /* 0: none                                                   */
+  int32_t sinks;
+  int32_t shared_len;
+  int32_t dtype;
+  float   softmax_scale;  /* <= 0 selects 1/sqrt(D)                                    */
+} MiniAttnCacheParams;
+
+/* scratch: as for miniattn_fwd_balanced, miniattn_fwd_cache_scratch_bytes(p) bytes; not optional.  That size depends on the
+ * sizes in `p` alone; pointers are compared with null and not read. */
+int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scratch_bytes, void* stream);
+int64_t miniattn_fwd_cache_scratch_bytes(const MiniAttnCacheParams* p);
+
+/*
+ * New tokens into a paged cache: k and v of token i of sequence b's n new ones go to position seq_lens[b] - n + i of the
+ * sequence (block table and caches as above), k rotated by that position, q rotated into q_out (which may be q).
+ *
+ * rope: [rope_rows, rot] fp32, the cosines of the rot / 2 angles of each position and then their sines; null: nothing is
+ * rotated.  Pairs are elements (i, i + rot / 2), with `interleaved` (2i, 2i + 1); elements from rot on stay as they are.
+ * Tokens before position 0 (the front of a padded sequence) are left out, their rows of q copied.  A position past the block
+ * table or the rotation table, or a page outside the cache, sets bit 7 of the status word; the token is left out.  Two tokens
+ * of one call must not go to the same place.
+ */
+typedef struct MiniAttnAppendParams {
+  const void* k;
+  const void* v;
+  const void* q;          /* optional                                                  */
+  void*       k_cache;
+  void*       v_cache;
+  void*       q_out;      /* not null with q                                           */
+  const float* rope;      /* optional                                                  */
+  int32_t*    status;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_q;    /* optional                                                  */
+  int64_t k_stride[3];    /* (sequence, head, token) of the new tokens                 */
+  int64_t v_stride[3];
+  int64_t q_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_cache_stride[3]; /* (page, head, token)                                    */
+  int64_t v_cache_stride[3];
+  int64_t table_stride;
+  int32_t B, Hq, Hkv, D;
+  int32_t n;              /* new tokens of each sequence, without cu_q                 */
+  int32_t total;          /* with cu_q: rows of k, v and q                             */
+  int32_t rot, interleaved, rope_rows;
+  int32_t page_size, n_pages, table_width;
+  int32_t dtype;
+} MiniAttnAppendParams;
+
+int miniattn_paged_append(const MiniAttnAppendParams* p, void* stream);
+
+/*
  * Failure-detection self-test (no reference counterpart; the reference never checks
  * its launches, flash_attention.cu:123).  Launches one CTA that waits on a barrier
  * nothing signals.  The wait gives up after `limit_ns` nanoseconds (0 < limit_ns <= 2e9),
@@ -305,7 +405,8 @@ int miniattn_selftest_wait(int32_t* status, uint64_t limit_ns, void* stream);
 
 /*
  * Turns a status word read back from the device (MiniAttnFwdParams.status, after synchronising)
- * into a return code: 0 when it is zero, MINIATTN_EDEVICE_WAIT otherwise, with the bounded waits
+ * into a return code: 0 when it is zero, MINIATTN_EINVAL where only bit 7 is set (a length, page or position
+ * of a paged call outside its tensors), MINIATTN_EDEVICE_WAIT otherwise, with the bounded waits
  * that ran out named in miniattn_last_error_string().  After such a failure the outputs of the
  * launches that shared the word are undefined, and the arrival counters of a balanced launch's
  * scratch may be non-zero: clear the word and the first 16384 bytes of that scratch before the

@@ -15,6 +15,8 @@
 #include <vector>
 
 #include "../../include/miniattn.h"
+#include "append.cuh"
+#include "cache.cuh"
 #include "common.cuh"
 #include "linear.cuh"
 
@@ -43,6 +45,9 @@ cudaError_t launch_quant_qk_static(int D, bool bf16, const void* q, const long l
                                    float q_fold, int8_t* q8, int8_t* k8, float* sq, float* sk,
                                    float* k_mean, cudaStream_t st);
 cudaError_t launch_linear(bool bf16, const LinearArgs& a, int pairs, cudaStream_t st);
+cudaError_t launch_fwd_cache(int D, bool bf16, const CUtensorMap* tm, const CacheArgs& a, int rg, int n_ctas,
+                             cudaStream_t st);
+cudaError_t launch_append(bool bf16, const AppendArgs& a, int sms, cudaStream_t st);
 cudaError_t launch_wait_selftest(int32_t* status, unsigned long long limit_ns, cudaStream_t st);
 cudaError_t launch_merge_partials(float* acc_o, float* acc_lse, const void* part_o,
                                   const float* part_lse, void* out, long long rows, int D, bool bf16,
@@ -966,11 +971,232 @@ int miniattn_linear(const MiniAttnLinearParams* p, void* stream) {
   return MINIATTN_OK;
 }
 
+// ---- attention over a cache, and what fills one ----
+static int page_shift_of(int page_size) {
+  for (int s = 4; s <= 10; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+
+static int check_table(const int32_t* table, int64_t stride, int width, int page_size, int n_pages, const int32_t* lens) {
+  if ((table == nullptr && width > 0) || lens == nullptr)
+    return fail(MINIATTN_EINVAL, "block_table and seq_lens must not be null");
+  if (page_shift_of(page_size) < 0)
+    return fail(MINIATTN_EUNSUPPORTED, "page size %d not supported (a power of two from 16 to 1024)", page_size);
+  if (width < 0 || n_pages < 0 || stride < width)
+    return fail(MINIATTN_EINVAL, "block table of %d columns %lld apart, %d pages", width, (long long)stride, n_pages);
+  if (reinterpret_cast<uintptr_t>(table) % 4 != 0 || reinterpret_cast<uintptr_t>(lens) % 4 != 0)
+    return fail(MINIATTN_EINVAL, "block_table and seq_lens must be 4-byte aligned");
+  return MINIATTN_OK;
+}
+
+// Returns 1 when there is nothing to do.
+static int check_cache_sizes(const MiniAttnCacheParams* p) {
+  if (p == nullptr) return fail(MINIATTN_EINVAL, "params is null");
+  if (p->dtype != MINIATTN_FP16 && p->dtype != MINIATTN_BF16)
+    return fail(MINIATTN_EUNSUPPORTED, "dtype must be fp16 (0) or bf16 (1), got %d", p->dtype);
+  if (p->D != 64 && p->D != 96 && p->D != 128)
+    return fail(MINIATTN_EUNSUPPORTED, "head dim %d not supported (64, 96 or 128)", p->D);
+  if (p->B < 0 || p->Hq < 0 || p->Hkv < 0 || p->Nq < 0 || p->Nk < 0 || p->total_q < 0)
+    return fail(MINIATTN_EINVAL, "negative size");
+  if (p->window < 0 || p->sinks < 0 || p->shared_len < 0) return fail(MINIATTN_EINVAL, "negative window, sinks or shared_len");
+  const long long rows = p->cu_q != nullptr ? p->total_q : static_cast<long long>(p->B) * p->Nq;
+  if (p->B == 0 || p->Hq == 0 || rows == 0) return 1;
+  if (p->Hkv == 0 || p->Hq % p->Hkv != 0)
+    return fail(MINIATTN_EINVAL, "Hq (%d) must be a positive multiple of Hkv (%d)", p->Hq, p->Hkv);
+  if (p->Hq > 65535 || p->B > 65535) return fail(MINIATTN_EUNSUPPORTED, "B and Hq must not exceed 65535");
+  if (rows > 0x7fffffff / p->Hq) return fail(MINIATTN_EUNSUPPORTED, "rows x heads must fit in 31 bits");
+  if (p->sinks > 0 && p->window == 0) return fail(MINIATTN_EINVAL, "sinks are what stays visible outside a window: window is 0");
+  if (p->page_size == 0) {
+    if (p->block_table != nullptr || p->seq_lens != nullptr || p->cu_q != nullptr || p->shared_len != 0)
+      return fail(MINIATTN_EINVAL, "block_table, seq_lens, cu_q and shared_len need pages");
+    if (p->diag > (1ll << 40) || p->diag < -(1ll << 40)) return fail(MINIATTN_EUNSUPPORTED, "positions beyond 2^40");
+    if (p->Nk > 0x7fffff00) return fail(MINIATTN_EUNSUPPORTED, "Nk (%d) is too large", p->Nk);
+  } else {
+    const int rc = check_table(p->block_table, p->table_stride, p->table_width, p->page_size, p->n_pages, p->seq_lens);
+    if (rc != 0) return rc;
+    if (p->shared_len % p->page_size != 0 || p->shared_len / p->page_size > p->table_width)
+      return fail(MINIATTN_EINVAL, "shared_len (%d) must be a multiple of the page size (%d) inside the block table",
+                  p->shared_len, p->page_size);
+    if (p->shared_len > 0 && p->window > 0)
+      return fail(MINIATTN_EUNSUPPORTED, "a shared prefix and a window do not go together");
+  }
+  return MINIATTN_OK;
+}
+
+namespace {
+struct CachePlan {
+  int rg, n_ctas;
+  size_t rows() const { return static_cast<size_t>(2 * n_ctas) * 16 * rg; }
+  size_t bytes(int D) const { return kCounterBytes + align256(rows() * sizeof(float2)) + rows() * kernel_head_dim(D) * sizeof(float); }
+};
+CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
+  const long long n = p->cu_q != nullptr && p->Nq == 0 ? p->total_q : p->Nq;
+  const long long rows = n * (p->Hq / p->Hkv);
+  return CachePlan{rows <= 16 ? 1 : rows <= 32 ? 2 : 4, 2 * sms};
+}
+}  // namespace
+
+int64_t miniattn_fwd_cache_scratch_bytes(const MiniAttnCacheParams* p) {
+  g_err[0] = 0;
+  int rc = check_cache_sizes(p), sms = 0;
+  if (rc == 1) return 0;
+  if (rc != 0 || (rc = check_device(&sms)) != 0) return rc;
+  return static_cast<int64_t>(cache_plan(p, sms).bytes(p->D));
+}
+
+int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scratch_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = check_cache_sizes(p);
+  if (rc != 0) return rc == 1 ? MINIATTN_OK : rc;
+  if ((rc = check_tensor(p->q, p->q_stride, p->D, "q")) != 0 || (rc = check_tensor(p->o, p->o_stride, p->D, "o")) != 0) return rc;
+  const bool paged = p->page_size != 0;
+  const bool has_keys = paged ? p->n_pages > 0 && p->table_width > 0 : p->Nk > 0;
+  if (has_keys && ((rc = check_tensor(p->k, p->k_stride, p->D, "k")) != 0 || (rc = check_tensor(p->v, p->v_stride, p->D, "v")) != 0))
+    return rc;
+  int sms = 0;
+  if ((rc = check_device(&sms)) != 0) return rc;
+  const CachePlan plan = cache_plan(p, sms);
+  if (scratch == nullptr || scratch_bytes < plan.bytes(p->D))
+    return fail(MINIATTN_EINVAL, "scratch holds %zu bytes, this launch needs %zu (miniattn_fwd_cache_scratch_bytes)",
+                scratch == nullptr ? size_t{0} : scratch_bytes, plan.bytes(p->D));
+  if (reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return fail(MINIATTN_EINVAL, "scratch must be 256-byte aligned");
+
+  ma::CacheArgs a{};
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.o = static_cast<uint16_t*>(p->o);
+  a.lse = p->lse;
+  a.status = p->status;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = i == 0 && p->cu_q != nullptr ? 0 : p->q_stride[i];
+    a.os[i] = i == 0 && p->cu_q != nullptr ? 0 : p->o_stride[i];
+  }
+  a.ls[0] = p->cu_q != nullptr ? 0 : p->lse_stride[0];
+  a.ls[1] = p->lse_stride[1];
+  a.table = p->block_table;
+  a.table_stride = p->table_stride;
+  a.seq_lens = p->seq_lens;
+  a.cu_q = p->cu_q;
+  a.diag = p->diag;
+  a.B = p->B;
+  a.Hq = p->Hq;
+  a.Hkv = p->Hkv;
+  a.G = p->Hq / p->Hkv;
+  a.D = p->D;
+  a.Nq = p->Nq;
+  a.Nk = p->Nk;
+  a.total_q = p->total_q;
+  a.page_shift = paged ? page_shift_of(p->page_size) : 0;
+  a.n_pages = p->n_pages;
+  a.table_width = p->n_pages > 0 ? p->table_width : 0;
+  a.window = p->window;
+  a.sinks = p->sinks;
+  a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / sqrtf((float)p->D)) * 1.4426950408889634f;
+  a.by_g = ma::fast_div(a.G);
+  a.by_hkv = ma::fast_div(a.Hkv);
+  a.by_nq = ma::fast_div(p->Nq > 0 ? p->Nq : 1);
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  a.counters = reinterpret_cast<int*>(base);
+  a.part_ml = reinterpret_cast<float2*>(base + kCounterBytes);
+  a.part_o = reinterpret_cast<float*>(base + kCounterBytes + align256(plan.rows() * sizeof(float2)));
+
+  const CUtensorMapDataType dt =
+      p->dtype == MINIATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tm[2] = {};
+  if (has_keys) {
+    const int n = paged ? p->page_size : p->Nk, box = paged ? std::min(64, p->page_size) : 64;
+    const int outer = paged ? p->n_pages : p->B;
+    if ((rc = make_map(&tm[0], p->k, 2, dt, p->D, n, p->Hkv, outer, p->k_stride, ma::kBoxCols, box, "k")) != 0 ||
+        (rc = make_map(&tm[1], p->v, 2, dt, p->D, n, p->Hkv, outer, p->v_stride, ma::kBoxCols, box, "v")) != 0)
+      return rc;
+  }
+  const cudaError_t e = ma::launch_fwd_cache(kernel_head_dim(p->D), p->dtype == MINIATTN_BF16, tm, a, plan.rg, plan.n_ctas,
+                                             reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(MINIATTN_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+  return MINIATTN_OK;
+}
+
+int miniattn_paged_append(const MiniAttnAppendParams* p, void* stream) {
+  g_err[0] = 0;
+  if (p == nullptr) return fail(MINIATTN_EINVAL, "params is null");
+  if (p->dtype != MINIATTN_FP16 && p->dtype != MINIATTN_BF16)
+    return fail(MINIATTN_EUNSUPPORTED, "dtype must be fp16 (0) or bf16 (1), got %d", p->dtype);
+  if (p->D != 64 && p->D != 96 && p->D != 128)
+    return fail(MINIATTN_EUNSUPPORTED, "head dim %d not supported (64, 96 or 128)", p->D);
+  if (p->B < 0 || p->Hq < 0 || p->Hkv < 0 || p->n < 0 || p->total < 0) return fail(MINIATTN_EINVAL, "negative size");
+  const long long rows = p->cu_q != nullptr ? p->total : static_cast<long long>(p->B) * p->n;
+  if (p->B == 0 || rows == 0) return MINIATTN_OK;
+  if (p->Hkv == 0) return fail(MINIATTN_EINVAL, "Hkv must be positive");
+  if (p->Hq > 65535 || p->Hkv > 65535 || p->B > 65535) return fail(MINIATTN_EUNSUPPORTED, "B, Hq and Hkv must not exceed 65535");
+  if (rows > 0x7fffffff) return fail(MINIATTN_EUNSUPPORTED, "the number of rows must fit in 31 bits");
+  int rc;
+  if ((rc = check_table(p->block_table, p->table_stride, p->table_width, p->page_size, p->n_pages, p->seq_lens)) != 0) return rc;
+  if (p->rope != nullptr) {
+    if (p->rot < 16 || p->rot > p->D || p->rot % 16 != 0)
+      return fail(MINIATTN_EUNSUPPORTED, "rot (%d) must be a multiple of 16 up to the head dim (%d)", p->rot, p->D);
+    if (p->rope_rows < 0) return fail(MINIATTN_EINVAL, "negative size");
+    if (reinterpret_cast<uintptr_t>(p->rope) % 16 != 0) return fail(MINIATTN_EINVAL, "rope must be 16-byte aligned");
+  }
+  if (p->interleaved != 0 && p->interleaved != 1) return fail(MINIATTN_EINVAL, "interleaved must be 0 or 1");
+  if ((rc = check_tensor(p->k, p->k_stride, p->D, "k")) != 0 || (rc = check_tensor(p->v, p->v_stride, p->D, "v")) != 0) return rc;
+  const bool has_q = p->q != nullptr && p->Hq > 0;
+  if (has_q && ((rc = check_tensor(p->q, p->q_stride, p->D, "q")) != 0 || (rc = check_tensor(p->q_out, p->q_out_stride, p->D, "q_out")) != 0))
+    return rc;
+  const bool has_pages = p->n_pages > 0 && p->table_width > 0;
+  if (has_pages && ((rc = check_tensor(p->k_cache, p->k_cache_stride, p->D, "k_cache")) != 0 ||
+                    (rc = check_tensor(p->v_cache, p->v_cache_stride, p->D, "v_cache")) != 0))
+    return rc;
+  int sms = 0;
+  if ((rc = check_device(&sms)) != 0) return rc;
+  ma::AppendArgs a{};
+  a.k = static_cast<const uint16_t*>(p->k);
+  a.v = static_cast<const uint16_t*>(p->v);
+  a.q = has_q ? static_cast<const uint16_t*>(p->q) : nullptr;
+  a.k_cache = static_cast<uint16_t*>(p->k_cache);
+  a.v_cache = static_cast<uint16_t*>(p->v_cache);
+  a.q_out = static_cast<uint16_t*>(p->q_out);
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = p->k_stride[i];
+    a.vs[i] = p->v_stride[i];
+    a.qs[i] = p->q_stride[i];
+    a.qos[i] = p->q_out_stride[i];
+    a.kcs[i] = p->k_cache_stride[i];
+    a.vcs[i] = p->v_cache_stride[i];
+  }
+  a.rope = p->rope;
+  a.table = p->block_table;
+  a.seq_lens = p->seq_lens;
+  a.cu_q = p->cu_q;
+  a.status = p->status;
+  a.table_stride = p->table_stride;
+  a.B = p->B;
+  a.n = p->n;
+  a.rows = static_cast<int>(rows);
+  a.Hq = p->Hq;
+  a.Hkv = p->Hkv;
+  a.D = p->D;
+  a.rot = p->rope != nullptr ? p->rot : 0;
+  a.interleaved = p->interleaved;
+  a.rope_rows = p->rope_rows;
+  a.page_shift = page_shift_of(p->page_size);
+  a.n_pages = p->n_pages;
+  a.table_width = has_pages ? p->table_width : 0;
+  a.by_n = ma::fast_div(p->n > 0 ? p->n : 1);
+  a.by_units = ma::fast_div(p->D / 16);
+  const cudaError_t e = ma::launch_append(p->dtype == MINIATTN_BF16, a, sms, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(MINIATTN_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+  return MINIATTN_OK;
+}
+
 int miniattn_check_status(int32_t status_word) {
   g_err[0] = 0;
   if (status_word == 0) return MINIATTN_OK;
   static const char* const names[] = {"K/V or Q tile load", "S = QK^T", "O += PV", "P hand-off", "ring slot release",
                                       "(bit 5, not in use)", "partial of another CTA of a cut item"};
+  constexpr int32_t kOutside = 1 << 7;
+  if (status_word == kOutside)
+    return fail(MINIATTN_EINVAL, "a length, page or position of a paged call lay outside its tensors (status word 0x%x)",
+                status_word);
   char list[256] = "";
   for (int bit = 0; bit < 7; ++bit)
     if (status_word & (1 << bit)) {

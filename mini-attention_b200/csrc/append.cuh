@@ -1,0 +1,58 @@
+// Appending new tokens to a paged cache: what the kernel and the host share.
+#pragma once
+#include <cstdint>
+
+#include "common.cuh"
+
+namespace ma {
+
+struct AppendArgs {
+  const uint16_t *k, *v, *q;       // new tokens; q may be null
+  uint16_t *k_cache, *v_cache, *q_out;
+  long long ks[3], vs[3], qs[3], qos[3];  // element strides: sequence, head, token (ragged: the first is 0)
+  long long kcs[3], vcs[3];        // element strides of the caches: page, head, token of the page
+  const float* rope;               // [rope_rows][rot]: cosines of the rot / 2 angles of a position, then their sines; or null
+  const int* table;                // [B][table_width] page numbers
+  const int* seq_lens;             // [B] tokens of each sequence, the new ones among them
+  const int* cu_q;                 // [B + 1] first row of each sequence; null: n rows each
+  int32_t* status;
+  long long table_stride;
+  int B, n, rows, Hq, Hkv, D;
+  int rot, interleaved, rope_rows;
+  int page_shift, n_pages, table_width;
+  FastDiv by_n, by_units;
+};
+
+// Sequence and position of row t.  False: the row belongs to no sequence, or its position lies before the sequence's first.
+struct AppendSlot {
+  bool held;            // the cache has a place for it
+  bool bad;             // a length, a page or a position outside the call's tensors
+  int pos;
+  long long page;       // page and token of the page, where held
+  int at;
+};
+// `first`: the sequence's first row, `n_new`: its rows.  The block table is looked up by the caller's function.
+template <typename Table>
+__host__ __device__ inline AppendSlot append_slot(const AppendArgs& a, int t, long long first, long long n_new, int seq_len,
+                                                  const Table& table) {
+  AppendSlot s{};
+  const long long pos = seq_len - n_new + (t - first);
+  const long long room = static_cast<long long>(a.table_width) << a.page_shift;
+  if (pos < 0) return s;  // the front of a padded sequence
+  if (pos >= room || (a.rope != nullptr && pos >= a.rope_rows)) {
+    s.bad = true;
+    return s;
+  }
+  s.pos = static_cast<int>(pos);
+  const int page = table(s.pos >> a.page_shift);
+  if (page < 0 || page >= a.n_pages) {
+    s.bad = true;
+    return s;
+  }
+  s.held = true;
+  s.page = page;
+  s.at = s.pos & ((1 << a.page_shift) - 1);
+  return s;
+}
+
+}  // namespace ma

@@ -1,0 +1,612 @@
+// Attention over a cache for few query rows per KV head (decode, drafts), and for any others.
+//
+// o_i = sum_j p_ij v_j / sum_j p_ij with p_ij = exp(s_ij - m_i) over the keys j that query token i sees: those up to its
+// own position, at most the last `window` of them and the first `sinks` ones.  K and V come through a block table (pages
+// of 16 to 1024 tokens in any order) or lie one after the other.  One pass over the keys with a running maximum and sum.
+//
+//   item      = (sequence, KV head, block of 16 * RG rows); a row is (token, query head of the KV head's G), so that K and V
+//               cross an SM once for all the heads that share them
+//   CTA       = a contiguous range of the 64-key tiles of all items, the same length for each: lengths are known on the GPU
+//               alone, so every CTA adds up the tiles of all sequences and finds its own
+//   warp 4    TMA producer: a copy per page (at most 64 keys) and 64 columns of K and of V, each issued by a lane of its own
+//   warps 0-3 16 rows x (16 * RG keys of the tile) each, running (m, l, O) in registers
+//
+// A CTA whose range cuts an item leaves its piece (un-normalised O, m, l) in scratch and counts itself in; the one that
+// counts in last folds the pieces, those that another launch left for these rows among them (a shared prefix).
+//
+// Keys that no row sees are never read: their pages may be gone or hold anything.  Where a tile holds some, their scores
+// are replaced and their rows of V cleared, so that what lies there does not reach a result.
+#include <atomic>
+#include <type_traits>
+
+#include "cache.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
+
+namespace ma {
+
+namespace {
+
+constexpr int kThreads = 160;
+constexpr int kKeys = 64;            // keys per tile
+constexpr int kBox = kKeys * 128;    // one [64 keys x 128 B] box
+constexpr float kLazy = 8.0f;        // log2 units a row's maximum may move before O is rescaled
+constexpr int kMergePitch = 36;      // floats per row of the merge buffer (32 + padding)
+
+template <int D>
+struct Layout {
+  static constexpr int kBoxes = D / 64;
+  static constexpr int kStageBytes = 2 * kBoxes * kBox;  // K then V
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kOffMerge = kStages * kStageBytes;              // float[4 warps][16][kMergePitch]
+  static constexpr int kOffMl = kOffMerge + 4 * 16 * kMergePitch * 4;  // float2[4 warps][16]
+  static constexpr int kOffBar = kOffMl + 4 * 16 * 8;                  // full[kStages], empty[kStages]
+  static constexpr int kOffScan = kOffBar + 2 * kStages * 8;           // long long[4 warps], start, total
+  static constexpr int kOffMisc = kOffScan + 6 * 8;                    // abort flag, arrival order, first sequence
+  static constexpr int kBytes = kOffMisc + 16;
+  static constexpr int kDynSmem = kBytes + 1024;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// weight of a partial with maximum m under the total maximum mt (0 for a partial without keys)
+__device__ __forceinline__ float part_weight(float m, float mt) { return m == -INFINITY ? 0.f : ex2(m - mt); }
+// natural logarithm of a row's sum; -inf where it saw no key, NaN where a score was one
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.f ? -INFINITY : m * 0.6931471805599453f + __logf(l);
+}
+
+// Sequence b of the call, and how its items are counted: n_rb row blocks per KV head, tiles of each.
+struct Walk {
+  CacheSeq s;
+  CacheTiles t;
+  int n_rb;
+  __device__ __forceinline__ long long total(const CacheArgs& a) const {
+    return static_cast<long long>(a.Hkv) * n_rb * t.n;
+  }
+};
+template <int kRows>
+__device__ __forceinline__ Walk walk_to(const CacheArgs& a, int b) {
+  Walk w;
+  int r0 = 0, r1 = 0;
+  if (a.cu_q != nullptr) {
+    r0 = a.cu_q[b];
+    r1 = a.cu_q[b + 1];
+  }
+  w.s = cache_seq(a, r0, r1, a.seq_lens != nullptr ? a.seq_lens[b] : 0);
+  w.t = cache_tiles<kKeys>(w.s.lo, w.s.hi, w.s.sink_end);
+  w.n_rb = static_cast<int>((static_cast<long long>(w.s.nq) * a.G + kRows - 1) / kRows);
+  return w;
+}
+
+}  // namespace
+
+template <int D, bool BF16, int RG>
+__global__ void __launch_bounds__(kThreads, 2)
+fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a,
+                 int min_share) {
+  using L = Layout<D>;
+  constexpr int KG = 4 / RG;      // key groups: warps that share a row group
+  constexpr int kRows = 16 * RG;  // rows of an item
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (sbase - raw);
+  const uint32_t bars = sbase + L::kOffBar;
+  auto full = [&](int s) -> uint32_t { return bars + 8u * s; };
+  auto empty = [&](int s) -> uint32_t { return bars + 8u * (L::kStages + s); };
+  long long* scan = reinterpret_cast<long long*>(gbase + L::kOffScan);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kOffMisc);
+  volatile int* order = abort_flag + 1;
+  int* first_seq = reinterpret_cast<int*>(gbase + L::kOffMisc) + 2;
+
+  grid_dep_launch();
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const WaitCtx wc{abort_flag, a.status, MINIATTN_WAIT_LIMIT_NS};
+  if (tid == 128) {
+    for (int s = 0; s < L::kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  grid_dep_wait();
+
+  // ---- this CTA's tiles [lo, hi) of the launch's total: each of 128 threads adds up a run of sequences ----
+  const int run = (a.B + 127) / 128;
+  const int b0 = min(a.B, tid * run), b1 = tid < 128 ? min(a.B, b0 + run) : b0;
+  long long mine = 0;
+  bool bad = false;
+  for (int b = b0; b < b1; ++b) {
+    const Walk w = walk_to<kRows>(a, b);
+    mine += w.total(a);
+    bad |= w.s.bad;
+  }
+  if (bad && a.status != nullptr) atomicOr(a.status, kErrCache);
+  long long before = mine;  // inclusive over the warp, then exclusive over the CTA
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += o;
+  }
+  if (lane == 31 && warp < 4) scan[warp] = before;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  before -= mine;
+  const long long n_ctas = gridDim.x;
+  const long long share = max(static_cast<long long>(min_share), (total + n_ctas - 1) / n_ctas);
+  const long long lo = blockIdx.x * share, hi = min(total, lo + share);
+  if (lo >= hi) return;
+  if (tid < 128 && lo >= before && lo < before + mine) {
+    int b = b0;
+    for (;; ++b) {
+      const long long n = walk_to<kRows>(a, b).total(a);
+      if (lo < before + n) break;
+      before += n;
+    }
+    *first_seq = b;
+    scan[4] = before;
+  }
+  __syncthreads();
+  int b = *first_seq;
+  long long base = scan[4];  // tiles before sequence b
+  Walk w = walk_to<kRows>(a, b);
+  auto next_seq = [&]() {  // the next sequence that has rows; only while tiles are left
+    do {
+      base += w.total(a);
+      w = walk_to<kRows>(a, ++b);
+    } while (w.n_rb == 0);
+  };
+
+  if (warp == 4) {
+    // =========================== TMA producer ====================================
+    // Lane l copies one box of a tile: page l / (2 * kBoxes) of it, K or V, 64 columns.  The page numbers of the next tile
+    // are fetched before the wait for its slot.
+    const int keys_shift = a.table != nullptr ? min(6, a.page_shift) : 6;  // keys of a box
+    const int n_lanes = (kKeys >> keys_shift) * 2 * L::kBoxes;
+    const int sub = lane / (2 * L::kBoxes), bx = lane % L::kBoxes;
+    const bool is_v = (lane / L::kBoxes) & 1;
+    const uint32_t dst = (is_v ? L::kBoxes * kBox : 0) + bx * kBox + ((sub << keys_shift) << 7);
+    const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
+    const uint32_t box_bytes = 128u << keys_shift;
+    int hk, j;
+    auto locate = [&](long long x) {
+      const long long within = x - base, it = within / w.t.n;
+      j = static_cast<int>(within - it * w.t.n);
+      hk = static_cast<int>(it / w.n_rb);
+      return static_cast<int>(it - static_cast<long long>(hk) * w.n_rb);
+    };
+    int rb = locate(lo);
+    int key = 0, page = 0;
+    bool wanted = false;
+    auto look_up = [&]() {  // the page of this lane's keys of tile j
+      key = w.t.at(j) * kKeys + (sub << keys_shift);
+      wanted = lane < n_lanes && cache_seen(w.s.lo, w.s.hi, w.s.sink_end, key, 1 << keys_shift);
+      page = b;
+      if (a.table != nullptr) {
+        if (wanted) page = a.table[b * a.table_stride + (key >> a.page_shift)];
+        key &= (1 << a.page_shift) - 1;
+        if (wanted && static_cast<unsigned>(page) >= static_cast<unsigned>(a.n_pages)) {
+          wanted = false;
+          if (a.status != nullptr) atomicOr(a.status, kErrCache);
+        }
+      }
+    };
+    look_up();
+    int slot = 0, par = 1, i = 0;
+    for (long long x = lo; x < hi; ++x, ++i) {
+      if (i >= L::kStages) mbar_wait(empty(slot), par, wc, kErrWaitFree);
+      const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, wanted));
+      if (lane == 0) mbar_expect_tx(full(slot), n_copies * box_bytes);
+      __syncwarp();
+      if (wanted) tma_load_4d(sbase + slot * L::kStageBytes + dst, tm, full(slot), bx * 64, key, hk, page);
+      __syncwarp();
+      if (++slot == L::kStages) {
+        slot = 0;
+        par ^= 1;
+      }
+      if (x + 1 < hi) {
+        if (++j == w.t.n) {
+          j = 0;
+          if (++rb == w.n_rb) {
+            rb = 0;
+            if (++hk == a.Hkv) {
+              hk = 0;
+              next_seq();
+            }
+          }
+        }
+        look_up();
+      }
+    }
+    // give-up path: let the copies in flight land (bounded) before the shared memory is released
+    if (*abort_flag) {
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 2000000ull) {
+      }
+    }
+    __syncwarp();
+    return;
+  }
+
+  // ---------------------------------------------------------------- workers
+  const int rg = warp % RG, kg = warp / RG;
+  const int g = lane >> 2, tig = lane & 3;
+  float* merge = reinterpret_cast<float*>(gbase + L::kOffMerge);
+  float2* ml_s = reinterpret_cast<float2*>(gbase + L::kOffMl);
+  const float c = a.scale_log2;
+  // ldmatrix row addresses: lanes 0-7 / 8-15 / 16-23 / 24-31 address the four 8x8 matrices
+  const int k_row = (lane & 7) + ((lane >> 4) << 3), k_chunk = (lane >> 3) & 1;  // K: keys x dims
+  const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_chunk = lane >> 4;  // V: trans
+  int slot = 0, par = 0;
+
+  for (long long x = lo; x < hi;) {
+    while (x >= base + w.total(a)) next_seq();
+    const long long it = (x - base) / w.t.n;
+    const long long item0 = base + it * w.t.n;
+    const int t0 = static_cast<int>(x - item0);
+    const int t1 = static_cast<int>(min(static_cast<long long>(w.t.n), hi - item0));
+    const int hk = static_cast<int>(it / w.n_rb), rb = static_cast<int>(it - static_cast<long long>(hk) * w.n_rb);
+    const int rows = w.s.nq * a.G, row0 = rb * kRows;
+
+    // Q fragments of this warp's 16 rows, and which keys its two rows of this lane see
+    uint32_t qf[D / 16][4];
+    int first[2], end[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = row0 + rg * 16 + g + 8 * e;
+      const int tok = div_by(r, a.by_g);
+      const bool ok = r < rows;
+      cache_row(a, w.s, tok, &first[e], &end[e]);
+      if (!ok) end[e] = 0;
+      const uint16_t* qp = a.q + b * a.qs[0] + (hk * a.G + (r - tok * a.G)) * a.qs[1] + (w.s.row0 + tok) * a.qs[2];
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const int col = ks * 16 + tig * 2;  // D = 96 runs on the D = 128 kernel: columns past it are 0
+        qf[ks][e] = (ok && col < a.D) ? *reinterpret_cast<const uint32_t*>(qp + col) : 0u;
+        qf[ks][2 + e] = (ok && col + 8 < a.D) ? *reinterpret_cast<const uint32_t*>(qp + col + 8) : 0u;
+      }
+    }
+    const int all_from = __reduce_max_sync(0xffffffffu, max(first[0], first[1]));
+    const int all_to = __reduce_min_sync(0xffffffffu, min(end[0], end[1]));
+
+    float acc[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+
+    for (int t = t0; t < t1; ++t) {
+      mbar_wait(full(slot), par, wc, kErrWaitKV);
+      const uint32_t sK = sbase + slot * L::kStageBytes;
+      const uint32_t sV = sK + L::kBoxes * kBox;
+      const int key0 = kg * kRows;  // this warp's keys of the tile: [key0, key0 + 16 * RG)
+      const int kbase = w.t.at(t) * kKeys + key0;
+      const bool some_hidden = kbase < all_from || kbase + kRows > all_to;
+      if (kbase + kRows > w.s.hi || kbase < w.s.lo) {
+        // Keys that no row sees: whatever lies in their rows of V (another sequence's, nothing yet, an infinity) must not
+        // meet their weight of 0.  Warps that share the keys write the same zeros.
+        uint8_t* rows_v = gbase + slot * L::kStageBytes + L::kBoxes * kBox;
+        for (int i = lane; i < kRows * 8 * L::kBoxes; i += 32) {
+          const int r = (i >> 3) % kRows, box = (i >> 3) / kRows;
+          if (!cache_seen(w.s.lo, w.s.hi, w.s.sink_end, kbase + r, 1))
+            *reinterpret_cast<uint4*>(rows_v + box * kBox + (key0 + r) * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();  // the slot's next copy comes after these writes
+        __syncwarp();
+      }
+      // All RG * 2 accumulator chains advance together, and with one row group each is cut in two: an mma.sync waits for
+      // the one before it on its chain.
+      constexpr int kSplit = RG == 1 ? 2 : 1;
+      float sp[kSplit][RG][2][4];
+#pragma unroll
+      for (int u = 0; u < kSplit; ++u)
+#pragma unroll
+        for (int kc = 0; kc < RG; ++kc)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sp[u][kc][0][e] = sp[u][kc][1][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+        for (int kc = 0; kc < RG; ++kc) {
+          const int r = key0 + kc * 16 + k_row;
+          uint32_t kb[4];
+          ldsm4(sK + r * 128 + (ks >> 2) * kBox + ((((ks & 3) * 2 + k_chunk) ^ (r & 7)) << 4), kb);
+          mma16816<BF16>(sp[ks % kSplit][kc][0], qf[ks], kb[0], kb[1]);
+          mma16816<BF16>(sp[ks % kSplit][kc][1], qf[ks], kb[2], kb[3]);
+        }
+      }
+      auto& s = sp[0];
+      if constexpr (kSplit == 2) {
+#pragma unroll
+        for (int kc = 0; kc < RG; ++kc)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[kc][0][e] += sp[kSplit - 1][kc][0][e];
+            s[kc][1][e] += sp[kSplit - 1][kc][1][e];
+          }
+      }
+      if (some_hidden) {  // by selection: what a hidden key's score holds does not matter
+#pragma unroll
+        for (int kc = 0; kc < RG; ++kc)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = kbase + kc * 16 + n * 8 + tig * 2 + (e & 1);
+              if (key >= end[e >> 1] || (key < first[e >> 1] && key >= a.sinks)) s[kc][n][e] = -INFINITY;
+            }
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int kc = 0; kc < RG; ++kc)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          mx[0] = fmax3(mx[0], s[kc][n][0], s[kc][n][1]);
+          mx[1] = fmax3(mx[1], s[kc][n][2], s[kc][n][3]);
+        }
+      bool moved = false;
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * c;
+        const float m_new = fmaxf(m_run[e], mx[e]);
+        alpha[e] = 1.f;
+        if (m_new - m_run[e] > kLazy) {  // also taken when the running maximum is -inf
+          alpha[e] = ex2(m_run[e] - m_new);
+          m_run[e] = m_new;
+          moved = true;
+        }
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+        l_run[0] *= alpha[0];
+        l_run[1] *= alpha[1];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          acc[n][0] *= alpha[0];
+          acc[n][1] *= alpha[0];
+          acc[n][2] *= alpha[1];
+          acc[n][3] *= alpha[1];
+        }
+      }
+      const float mc0 = m_run[0] == -INFINITY ? 0.f : m_run[0];
+      const float mc1 = m_run[1] == -INFINITY ? 0.f : m_run[1];
+#pragma unroll
+      for (int kc = 0; kc < RG; ++kc) {
+        uint32_t pf[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = ex2(fmaf(s[kc][n][0], c, -mc0)), p1 = ex2(fmaf(s[kc][n][1], c, -mc0));
+          const float p2 = ex2(fmaf(s[kc][n][2], c, -mc1)), p3 = ex2(fmaf(s[kc][n][3], c, -mc1));
+          l_run[0] += p0 + p1;
+          l_run[1] += p2 + p3;
+          // P in 16 bits for the second product: off by half a step of the type for each weight
+          pf[2 * n] = pack2<BF16>(p0, p1);
+          pf[2 * n + 1] = pack2<BF16>(p2, p3);
+        }
+        const int r = key0 + kc * 16 + v_row;
+        const uint32_t rowa = sV + r * 128;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          uint32_t vb[4];
+          ldsm4_t(rowa + (n >> 2) * kBox + ((((n & 3) * 2 + v_chunk) ^ (r & 7)) << 4), vb);
+          mma16816<BF16>(acc[2 * n], pf, vb[0], vb[1]);
+          mma16816<BF16>(acc[2 * n + 1], pf, vb[2], vb[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty(slot));
+      if (++slot == L::kStages) {
+        slot = 0;
+        par ^= 1;
+      }
+    }
+
+    // ---- end of a piece: fold the key groups, then write the rows or publish the partial ----
+    const bool all_tiles = t0 == 0 && t1 == w.t.n;
+    const bool whole = all_tiles && a.n_ext == 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
+      if (tig == 0) ml_s[warp * 16 + g + 8 * e] = make_float2(m_run[e], l_run[e]);
+    }
+    workers_sync();
+    float f[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) mt = fmaxf(mt, ml_s[(k * RG + rg) * 16 + g + 8 * e].x);
+#pragma unroll
+      for (int k = 0; k < KG; ++k) {
+        const float2 ml = ml_s[(k * RG + rg) * 16 + g + 8 * e];
+        lt += ml.y * part_weight(ml.x, mt);
+      }
+      f[e] = part_weight(m_run[e], mt);
+      if (whole) f[e] *= lt > 0.f ? 1.f / lt : lt;  // a NaN stays one
+    }
+    const long long c_first = item0 / share;  // CTA that holds the item's first tile
+    const long long my_slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
+    auto lse_at = [&](int r) -> float* {
+      const int tok = div_by(r, a.by_g), h = hk * a.G + (r - tok * a.G);
+      return a.lse + b * a.ls[0] + h * a.ls[1] + w.s.row0 + tok;
+    };
+    if (tid < kRows && row0 + tid < rows) {
+      const int rgi = tid >> 4, rr = tid & 15;
+      float mt = -INFINITY, lt = 0.f;
+      for (int k = 0; k < KG; ++k) mt = fmaxf(mt, ml_s[(k * RG + rgi) * 16 + rr].x);
+      for (int k = 0; k < KG; ++k) {
+        const float2 ml = ml_s[(k * RG + rgi) * 16 + rr];
+        lt += ml.y * part_weight(ml.x, mt);
+      }
+      if (!whole) a.part_ml[my_slot * kRows + tid] = make_float2(mt, lt);
+      else if (a.lse != nullptr) *lse_at(row0 + tid) = row_lse(mt, lt);
+    }
+    auto store_row = [&](int r_in, int col, const float4& o) {  // four columns of a finished row
+      const int r = row0 + r_in, tok = div_by(r, a.by_g), h = hk * a.G + (r - tok * a.G);
+      uint2 y;
+      y.x = pack2<BF16>(o.x, o.y);
+      y.y = pack2<BF16>(o.z, o.w);
+      *reinterpret_cast<uint2*>(a.o + b * a.os[0] + h * a.os[1] + (w.s.row0 + tok) * a.os[2] + col) = y;
+    };
+#pragma unroll
+    for (int p = 0; p < D / 32; ++p) {  // 32 columns at a time through 9 KB
+      float* mine_s = merge + warp * 16 * kMergePitch;
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+        const int n = p * 4 + jj;
+        *reinterpret_cast<float2*>(mine_s + g * kMergePitch + jj * 8 + tig * 2) =
+            make_float2(acc[n][0] * f[0], acc[n][1] * f[0]);
+        *reinterpret_cast<float2*>(mine_s + (g + 8) * kMergePitch + jj * 8 + tig * 2) =
+            make_float2(acc[n][2] * f[1], acc[n][3] * f[1]);
+      }
+      workers_sync();
+      const int rr = tid >> 3, c4 = (tid & 7) * 4;
+#pragma unroll
+      for (int rgi = 0; rgi < RG; ++rgi) {
+        const int r_in = rgi * 16 + rr;
+        if (row0 + r_in >= rows) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < KG; ++k) {
+          const float4 y = *reinterpret_cast<const float4*>(merge + ((k * RG + rgi) * 16 + rr) * kMergePitch + c4);
+          o.x += y.x;
+          o.y += y.y;
+          o.z += y.z;
+          o.w += y.w;
+        }
+        const int col = p * 32 + c4;
+        if (!whole) *reinterpret_cast<float4*>(a.part_o + (my_slot * kRows + r_in) * D + col) = o;
+        else if (col < a.D) store_row(r_in, col, o);
+      }
+      workers_sync();
+    }
+    if (!whole) {
+      int n_parts = 1;
+      if (!all_tiles) {
+        __threadfence();  // release: the piece before the count
+        workers_sync();
+        n_parts = static_cast<int>((item0 + w.t.n - 1) / share - c_first + 1);
+        if (tid == 0) {
+          __threadfence();
+          *order = atomicAdd(a.counters + c_first, 1);
+        }
+        workers_sync();
+      } else {
+        __threadfence();  // the CTA reads its own piece back
+        workers_sync();
+      }
+      if (all_tiles || *order == n_parts - 1) {
+        __threadfence();  // acquire: every other piece was published before it was counted
+        if (!all_tiles && tid == 0) a.counters[c_first] = 0;
+        const int n_rows = min(kRows, rows - row0), n_all = n_parts + a.n_ext;
+        const long long ext_rows = (a.cu_q != nullptr ? a.total_q : static_cast<long long>(a.B) * a.Nq) * a.Hq;
+        // where piece p of a row lies: its own launch's pieces, then the other launch's
+        auto piece = [&](int p, int r_in, const float2** ml, const float** o) {
+          if (p < n_parts) {
+            const long long i = (2 * (c_first + p) + (p == 0 ? 1 : 0)) * kRows + r_in;
+            *ml = a.part_ml + i;
+            *o = a.part_o + i * D;
+          } else {
+            const int r = row0 + r_in, tok = div_by(r, a.by_g), h = hk * a.G + (r - tok * a.G);
+            const long long q_row = a.cu_q != nullptr ? w.s.row0 + tok : static_cast<long long>(b) * a.Nq + tok;
+            const long long i = (p - n_parts) * ext_rows + q_row * a.Hq + h;
+            *ml = a.ext_ml + i;
+            *o = a.ext_o + i * D;
+          }
+        };
+        const int n_el = n_rows * (D / 4);
+        for (int e = tid; e < n_el; e += 128) {
+          const int r_in = e / (D / 4), col = (e % (D / 4)) * 4;
+          const float2* ml;
+          const float* po;
+          float mt = -INFINITY, lt = 0.f;
+          for (int p = 0; p < n_all; ++p) {
+            piece(p, r_in, &ml, &po);
+            mt = fmaxf(mt, __ldcg(ml).x);
+          }
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int p = 0; p < n_all; ++p) {
+            piece(p, r_in, &ml, &po);
+            const float2 x2 = __ldcg(ml);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(po + col));
+            const float wgt = part_weight(x2.x, mt);
+            lt = fmaf(x2.y, wgt, lt);
+            o.x = fmaf(y.x, wgt, o.x);
+            o.y = fmaf(y.y, wgt, o.y);
+            o.z = fmaf(y.z, wgt, o.z);
+            o.w = fmaf(y.w, wgt, o.w);
+          }
+          const float inv = lt > 0.f ? 1.f / lt : lt;
+          o.x *= inv;
+          o.y *= inv;
+          o.z *= inv;
+          o.w *= inv;
+          if (col < a.D) store_row(r_in, col, o);
+          if (col == 0 && a.lse != nullptr) *lse_at(row0 + r_in) = row_lse(mt, lt);
+        }
+      }
+      workers_sync();  // `order` may be written again only when everyone has read it
+    }
+    x = item0 + t1;
+  }
+}
+
+// ---------------------------------------------------------------------------------
+template <int D, bool BF16, int RG>
+static cudaError_t launch_t(const CUtensorMap* tm, const CacheArgs& a, int n_ctas, cudaStream_t st) {
+  auto kern = fwd_cache_kernel<D, BF16, RG>;
+  static std::atomic<unsigned long long> smem_set{0};
+  cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kern), Layout<D>::kDynSmem, &smem_set);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(kern, n_ctas, kThreads, Layout<D>::kDynSmem, st, tm[0], tm[1], a, 4);
+}
+
+template <int D, bool BF16>
+static cudaError_t launch_d(const CUtensorMap* tm, const CacheArgs& a, int rg, int n_ctas, cudaStream_t st) {
+  if (rg == 1) return launch_t<D, BF16, 1>(tm, a, n_ctas, st);
+  if (rg == 2) return launch_t<D, BF16, 2>(tm, a, n_ctas, st);
+  return launch_t<D, BF16, 4>(tm, a, n_ctas, st);
+}
+
+// tm[0], tm[1]: K and V maps with boxes of 64 columns x min(64, page size) keys.
+cudaError_t launch_fwd_cache(int D, bool bf16, const CUtensorMap* tm, const CacheArgs& a, int rg, int n_ctas,
+                             cudaStream_t st) {
+  if (D == 128) return bf16 ? launch_d<128, true>(tm, a, rg, n_ctas, st) : launch_d<128, false>(tm, a, rg, n_ctas, st);
+  if (D == 64) return bf16 ? launch_d<64, true>(tm, a, rg, n_ctas, st) : launch_d<64, false>(tm, a, rg, n_ctas, st);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace ma

@@ -20,6 +20,7 @@ constexpr int kErrWaitP    = 1 << 3;   // P tile never published by the softmax 
 constexpr int kErrWaitFree = 1 << 4;   // a ring slot was never released
 // 1 << 5 was a hand-off between roles that no longer exist; nothing raises it
 constexpr int kErrWaitPeer = 1 << 6;   // another CTA of a cut work item never published its partial
+constexpr int kErrCache    = 1 << 7;   // a length, page or position of a paged call lies outside its tensors
 constexpr int kErrTest     = 1 << 30;  // raised only by the wait self-test kernel
 
 #ifndef MINIATTN_WAIT_LIMIT_NS

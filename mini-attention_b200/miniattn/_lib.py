@@ -93,6 +93,37 @@ class LinearParams(C.Structure):
     ]
 
 
+class CacheParams(C.Structure):
+    """Mirror of ``MiniAttnCacheParams``."""
+
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("status", C.c_void_p), ("block_table", C.c_void_p), ("seq_lens", C.c_void_p), ("cu_q", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3),
+        ("lse_stride", C.c_int64 * 2), ("table_stride", C.c_int64), ("diag", C.c_int64),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("Nq", C.c_int32),
+        ("total_q", C.c_int32), ("Nk", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+        ("table_width", C.c_int32), ("window", C.c_int32), ("sinks", C.c_int32), ("shared_len", C.c_int32),
+        ("dtype", C.c_int32), ("softmax_scale", C.c_float),
+    ]
+
+
+class AppendParams(C.Structure):
+    """Mirror of ``MiniAttnAppendParams``."""
+
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+        ("q_out", C.c_void_p), ("rope", C.c_void_p), ("status", C.c_void_p), ("block_table", C.c_void_p),
+        ("seq_lens", C.c_void_p), ("cu_q", C.c_void_p),
+        ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("q_stride", C.c_int64 * 3),
+        ("q_out_stride", C.c_int64 * 3), ("k_cache_stride", C.c_int64 * 3), ("v_cache_stride", C.c_int64 * 3),
+        ("table_stride", C.c_int64),
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("n", C.c_int32), ("total", C.c_int32),
+        ("rot", C.c_int32), ("interleaved", C.c_int32), ("rope_rows", C.c_int32), ("page_size", C.c_int32),
+        ("n_pages", C.c_int32), ("table_width", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
 def _load() -> C.CDLL:
     if not _LIB_PATH.exists():
         raise ImportError(
@@ -120,6 +151,12 @@ def _load() -> C.CDLL:
         getattr(lib, name).restype = C.c_int
     lib.miniattn_linear.argtypes = [C.c_void_p, C.c_void_p]   # a LinearParams by reference, or its bytes
     lib.miniattn_linear.restype = C.c_int
+    lib.miniattn_fwd_cache.argtypes = [C.POINTER(CacheParams), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.miniattn_fwd_cache.restype = C.c_int
+    lib.miniattn_fwd_cache_scratch_bytes.argtypes = [C.POINTER(CacheParams)]
+    lib.miniattn_fwd_cache_scratch_bytes.restype = C.c_int64
+    lib.miniattn_paged_append.argtypes = [C.POINTER(AppendParams), C.c_void_p]
+    lib.miniattn_paged_append.restype = C.c_int
     lib.miniattn_merge_partials.argtypes = [C.POINTER(MergeParams), C.c_void_p]
     lib.miniattn_merge_partials.restype = C.c_int
     lib.miniattn_selftest_wait.argtypes = [C.c_void_p, C.c_uint64, C.c_void_p]

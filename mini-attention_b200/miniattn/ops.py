@@ -195,6 +195,8 @@ def flash_attn_fwd(
     carry_in: bool = False,
     carry_out: bool = False,
     carry_rows: Optional[Tuple[int, int]] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ):
     """O = softmax(Q K^T * scale [+ causal mask]) V on the GPU.
 
@@ -216,10 +218,18 @@ def flash_attn_fwd(
     ``carry_rows=(first_row, total_rows)``: the buffer was made for a longer q of `total_rows` rows and
     this call's q is the row range of it that starts at `first_row` (a multiple of 128).
 
+    ``window`` (with ``causal``): a query sees the keys up to its own position, of them the last ``window``
+    (key j iff ``k_pos0 + j > q_pos0 + i - window``) and those at the first ``sinks`` positions
+    (``k_pos0 + j < sinks``).  Not together with ``carry``; ``balance`` has no say.
+
     The launch is asynchronous.  Every device-side wait is bounded; one that runs out sets a bit in a
     per-device status word instead of hanging — poll it with :func:`check_device_status` /
     :func:`device_status` after synchronising.
     """
+    if window is not None or sinks:
+        if carry is not None or carry_in or carry_out or carry_rows is not None:
+            raise RuntimeError("a window and a carried state do not go together")
+        return _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q_pos0, k_pos0, window, sinks)
     use_carry = bool(carry_in or carry_out)
     if use_carry and carry is None:
         raise RuntimeError("carry_in / carry_out need a carry buffer (carry_state)")
@@ -293,6 +303,85 @@ def flash_attn_fwd(
     if carry_out:
         return None
     return (out, lse) if return_lse else out
+
+
+_INT32_MAX = 2 ** 31 - 1
+_window_params: dict = {}   # parameter blocks of recent calls with a window, as _param_cache
+
+
+def _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q_pos0, k_pos0, window, sinks):
+    """``flash_attn_fwd`` with a sliding window."""
+    try:
+        key = (q.data_ptr(), k.data_ptr(), v.data_ptr(), q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype,
+               k.dtype, v.dtype, q.get_device(), k.get_device(), v.get_device(),
+               None if out is None else (out.data_ptr(), out.shape, out.stride(), out.dtype, out.get_device()), causal,
+               softmax_scale, layout, return_lse, kernel, q_pos0, k_pos0, window, sinks)
+        hit = _window_params.get(key)
+    except (AttributeError, TypeError, RuntimeError):
+        key = hit = None
+    if hit is None:
+        if window is None:
+            raise RuntimeError("sinks are what stays visible outside a window: window is None")
+        if not causal:
+            raise RuntimeError("a window needs causal=True")
+        if kernel != "auto":
+            raise RuntimeError("a window needs kernel='auto'")
+        if not 1 <= window <= _INT32_MAX or not 0 <= sinks <= _INT32_MAX:
+            raise RuntimeError(f"window must be positive and sinks not negative, got {window} and {sinks}")
+        f, out_f, lse_f = _prepare(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q_pos0, k_pos0)
+        if f is None:
+            return (out_f, lse_f) if return_lse else out_f
+        if max(*q.shape, *k.shape) > _INT32_MAX:
+            raise RuntimeError("sizes must fit in 31 bits")
+        p = _lib.CacheParams()
+        p.q, p.k, p.v, p.o, p.status = f.q, f.k, f.v, f.o if out is not None else None, f.status
+        p.q_stride[:], p.k_stride[:], p.v_stride[:], p.o_stride[:] = f.q_stride, f.k_stride, f.v_stride, f.o_stride
+        p.lse_stride[:] = (f.Hq * f.Nq, f.Nq)
+        p.diag = f.q_pos0 - f.k_pos0
+        p.B, p.Hq, p.Hkv, p.D, p.Nq, p.Nk = f.B, f.Hq, f.Hkv, f.D, f.Nq, f.Nk
+        p.window, p.sinks = int(window), max(0, min(_INT32_MAX, int(sinks) - f.k_pos0))
+        p.dtype, p.softmax_scale = f.dtype, f.softmax_scale
+        hit = (p, _cache_scratch_bytes(p, q.device))
+        if len(_window_params) >= _PARAM_CACHE_MAX:
+            _window_params.clear()
+        if key is not None:
+            _window_params[key] = hit
+    p, need = hit
+    if out is None or return_lse:
+        p = _lib.CacheParams.from_buffer_copy(p)   # the block that is kept stays as it is
+        if out is None:
+            out = torch.empty_like(q)
+            p.o = out.data_ptr()
+    lse = None
+    if return_lse:
+        lse = torch.empty((p.B, p.Hq, p.Nq), dtype=torch.float32, device=q.device)
+        p.lse = lse.data_ptr()
+    _launch_cache(p, need, q.device)
+    return (out, lse) if return_lse else out
+
+
+def _cache_scratch_bytes(p, device: torch.device) -> int:
+    with torch.cuda.device(device):
+        need = int(_lib.lib.miniattn_fwd_cache_scratch_bytes(_byref(p)))
+    if need < 0:
+        _lib.check(need, "miniattn_fwd_cache_scratch_bytes")
+    return need
+
+
+def _launch_cache(p, need: int, device: torch.device) -> None:
+    """``miniattn_fwd_cache`` on the current stream of `device`, with the scratch of that stream."""
+    if _current_device() == device.index:
+        rc = _launch_cache_on(p, need, device, _current_raw_stream(device.index))
+    else:
+        with torch.cuda.device(device.index):
+            rc = _launch_cache_on(p, need, device, _current_raw_stream(device.index))
+    if rc != _lib.OK:
+        _lib.check(rc, "miniattn_fwd_cache")
+
+
+def _launch_cache_on(p, need: int, device: torch.device, stream: int) -> int:
+    scratch = _scratch_for(device, stream, need)
+    return _lib.lib.miniattn_fwd_cache(_byref(p), scratch.data_ptr(), scratch.numel(), stream)
 
 
 # cudaStream_t of torch's current stream on a device without building a Stream object, and the current device
@@ -555,7 +644,6 @@ def selftest_wait(limit_ms: float = 50.0, device: Union[torch.device, str, None]
     return int(status.item())
 
 
-_INT32_MAX = 2 ** 31 - 1
 _Linear, _Parameter = torch.nn.Linear, torch.nn.Parameter
 _nn_module = torch.nn.modules.module
 _forward_ad = torch.autograd.forward_ad
