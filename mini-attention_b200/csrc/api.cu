@@ -47,6 +47,8 @@ cudaError_t launch_quant_qk_static(int D, bool bf16, const void* q, const long l
 cudaError_t launch_linear(bool bf16, const LinearArgs& a, int pairs, cudaStream_t st);
 cudaError_t launch_fwd_cache(int D, bool bf16, const CUtensorMap* tm, const CacheArgs& a, int rg, int n_ctas,
                              cudaStream_t st);
+cudaError_t launch_fwd_cache_ws(int D, bool bf16, bool prefix, const CUtensorMap* tm, const CacheArgs& a, int items, int parts,
+                                cudaStream_t st);
 cudaError_t launch_append(bool bf16, const AppendArgs& a, int sms, cudaStream_t st);
 cudaError_t launch_wait_selftest(int32_t* status, unsigned long long limit_ns, cudaStream_t st);
 cudaError_t launch_merge_partials(float* acc_o, float* acc_lse, const void* part_o,
@@ -1025,15 +1027,75 @@ static int check_cache_sizes(const MiniAttnCacheParams* p) {
 }
 
 namespace {
+// Which kernels a call over a cache runs.  Decided by sizes alone: lengths are known on the device only.
 struct CachePlan {
+  // rows of all sequences: fwd_cache.cu with rg groups of 16 rows, or (rg = 0) fwd_cache_ws.cu in `items` x `parts` CTAs
   int rg, n_ctas;
-  size_t rows() const { return static_cast<size_t>(2 * n_ctas) * 16 * rg; }
-  size_t bytes(int D) const { return kCounterBytes + align256(rows() * sizeof(float2)) + rows() * kernel_head_dim(D) * sizeof(float); }
+  int items, parts, pairs;
+  // a launch over the shared prefix before it: items x pieces of each
+  int pre_items, pre_parts, pre_pairs;
+  int pack, tpt, groups;
+  size_t part_rows, ext_rows;
+  size_t bytes(int D) const {
+    const size_t row = kernel_head_dim(D) * sizeof(float);
+    return kCounterBytes + align256(part_rows * sizeof(float2)) + align256(part_rows * row) +
+           align256(ext_rows * sizeof(float2)) + ext_rows * row;
+  }
 };
+
+constexpr int kMinPieceTiles = 4;  // 128-key tiles of a piece
+constexpr long long kMaxPieces = 480;  // of all items together: 64 MB of scratch at D = 128
+
+// Pieces that items of at most `tiles` tiles are cut into.  A CTA takes its tiles and about 4 steps of a tile's time beside
+// them; a piece takes 2 more to leave its result, the last 0.8 for each piece it folds.
+int cache_pieces(long long items, int tiles, int sms) {
+  int best = 1;
+  float least = 0.f;
+  for (int n = 1; n <= 32 && (n == 1 || (n * items <= kMaxPieces && tiles / n >= kMinPieceTiles)); ++n) {
+    const float rounds = static_cast<float>((items * n + sms - 1) / sms);
+    const float cost = rounds * (static_cast<float>((tiles + n - 1) / n) + 4.f + (n > 1 ? 2.f + 0.8f * n : 0.f));
+    if (n == 1 || cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
+}
+
 CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
-  const long long n = p->cu_q != nullptr && p->Nq == 0 ? p->total_q : p->Nq;
-  const long long rows = n * (p->Hq / p->Hkv);
-  return CachePlan{rows <= 16 ? 1 : rows <= 32 ? 2 : 4, 2 * sms};
+  CachePlan c{};
+  const bool ragged = p->cu_q != nullptr;
+  const int G = p->Hq / p->Hkv;
+  const long long n = ragged && p->Nq == 0 ? p->total_q : p->Nq, rows = n * G;
+  c.pack = G <= ma::kTileM ? G : 1;
+  c.tpt = ma::kTileM / c.pack;
+  c.groups = p->Hq / c.pack;
+  const int span = 2 * c.tpt;
+  const long long room = p->page_size != 0 ? static_cast<long long>(p->table_width) * p->page_size : p->Nk;
+  const auto tiles_of = [](long long keys) { return static_cast<int>(std::min<long long>((keys + 127) / 128, 1 << 24)); };
+  if (rows <= 32) {
+    c.rg = rows <= 16 ? 1 : 2;
+    c.n_ctas = 2 * sms;
+    c.part_rows = static_cast<size_t>(2 * c.n_ctas) * 16 * c.rg;
+    const bool stacked = ragged || p->Nq == 1 || p->q_stride[0] == p->Nq * p->q_stride[2];
+    if (p->shared_len > 0 && stacked) {
+      const long long all = ragged ? p->total_q : static_cast<long long>(p->B) * p->Nq;
+      c.pre_pairs = static_cast<int>((all + span - 1) / span);
+      c.pre_items = c.pre_pairs * c.groups;
+      const int tiles = tiles_of(p->shared_len);
+      c.pre_parts = std::max(1, std::min<int>(sms / std::max(c.pre_items, 1), tiles / kMinPieceTiles));
+      c.ext_rows = static_cast<size_t>(all) * p->Hq * c.pre_parts;
+    }
+    return c;
+  }
+  c.pairs = static_cast<int>((n + span - 1) / span);
+  const long long items = (ragged ? p->total_q / span + p->B : static_cast<long long>(p->B) * c.pairs) * c.groups;
+  const long long likely = ragged ? (p->total_q / span + (p->B + 1) / 2) * c.groups : items;
+  c.items = static_cast<int>(std::min<long long>(items, 0x7fffffff));
+  const long long seen = p->window > 0 ? std::min(room, static_cast<long long>(p->window) + p->sinks + span + 256) : room;
+  c.parts = items <= 2000 ? cache_pieces(std::max<long long>(likely, 1), tiles_of(seen), sms) : 1;
+  if (c.parts > 1) c.part_rows = static_cast<size_t>(items) * c.parts * 2 * ma::kTileM;
+  return c;
 }
 }  // namespace
 
@@ -1043,6 +1105,20 @@ int64_t miniattn_fwd_cache_scratch_bytes(const MiniAttnCacheParams* p) {
   if (rc == 1) return 0;
   if (rc != 0 || (rc = check_device(&sms)) != 0) return rc;
   return static_cast<int64_t>(cache_plan(p, sms).bytes(p->D));
+}
+
+// Maps of a launch of fwd_cache_ws.cu: q and o with `outer` sequences of n rows each.
+static int cache_ws_maps(const MiniAttnCacheParams* p, const CachePlan& c, CUtensorMapDataType dt, bool stacked, CUtensorMap* tm) {
+  const int n = stacked ? (p->cu_q != nullptr ? p->total_q : p->B * p->Nq) : p->Nq, outer = stacked ? 1 : p->B;
+  int64_t qs[3] = {p->q_stride[0], p->q_stride[1], p->q_stride[2]}, os[3] = {p->o_stride[0], p->o_stride[1], p->o_stride[2]};
+  if (stacked && p->cu_q == nullptr && p->Nq == 1) qs[2] = p->q_stride[0];  // a token each: their stride is the sequences'
+  if (stacked) qs[0] = os[0] = n * qs[2];
+  int rc;
+  if ((rc = make_map_packed(&tm[0], p->q, dt, p->D, n, c.groups, outer, qs, c.pack, c.tpt, "q")) != 0) return rc;
+  const bool boxes = ma::kWarpRows % c.pack == 0;  // otherwise rows of o are stored one by one
+  return boxes && (!stacked || p->cu_q != nullptr)
+             ? make_map_packed(&tm[3], p->o, dt, p->D, n, c.groups, outer, os, c.pack, ma::kWarpRows / c.pack, "o")
+             : MINIATTN_OK;
 }
 
 int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scratch_bytes, void* stream) {
@@ -1093,25 +1169,53 @@ int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scrat
   a.sinks = p->sinks;
   a.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / sqrtf((float)p->D)) * 1.4426950408889634f;
   a.by_g = ma::fast_div(a.G);
-  a.by_hkv = ma::fast_div(a.Hkv);
   a.by_nq = ma::fast_div(p->Nq > 0 ? p->Nq : 1);
-  uint8_t* base = static_cast<uint8_t*>(scratch);
-  a.counters = reinterpret_cast<int*>(base);
-  a.part_ml = reinterpret_cast<float2*>(base + kCounterBytes);
-  a.part_o = reinterpret_cast<float*>(base + kCounterBytes + align256(plan.rows() * sizeof(float2)));
+  const int Dk = kernel_head_dim(p->D);
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  a.counters = reinterpret_cast<int*>(at);
+  a.part_ml = reinterpret_cast<float2*>(at += kCounterBytes);
+  a.part_o = reinterpret_cast<float*>(at += align256(plan.part_rows * sizeof(float2)));
+  a.ext_ml = reinterpret_cast<float2*>(at += align256(plan.part_rows * Dk * sizeof(float)));
+  a.ext_o = reinterpret_cast<float*>(at += align256(plan.ext_rows * sizeof(float2)));
+  a.pack = plan.pack;
+  a.tpt = plan.tpt;
+  a.groups = plan.groups;
+  a.min_tiles = kMinPieceTiles;
+  a.by_pack = ma::fast_div(plan.pack);
+  a.by_groups = ma::fast_div(plan.groups);
+  a.by_gqa = ma::fast_div(a.G / plan.pack);
+  a.shared = p->shared_len;
 
-  const CUtensorMapDataType dt =
-      p->dtype == MINIATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap tm[2] = {};
-  if (has_keys) {
-    const int n = paged ? p->page_size : p->Nk, box = paged ? std::min(64, p->page_size) : 64;
+  const bool bf16 = p->dtype == MINIATTN_BF16;
+  const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const auto kv_maps = [&](CUtensorMap* tm, int most) {  // boxes of at most `most` keys
+    if (!has_keys) return 0;
+    const int n = paged ? p->page_size : p->Nk, box = paged ? std::min(most, p->page_size) : most;
     const int outer = paged ? p->n_pages : p->B;
-    if ((rc = make_map(&tm[0], p->k, 2, dt, p->D, n, p->Hkv, outer, p->k_stride, ma::kBoxCols, box, "k")) != 0 ||
-        (rc = make_map(&tm[1], p->v, 2, dt, p->D, n, p->Hkv, outer, p->v_stride, ma::kBoxCols, box, "v")) != 0)
-      return rc;
+    const int r = make_map(&tm[0], p->k, 2, dt, p->D, n, p->Hkv, outer, p->k_stride, ma::kBoxCols, box, "k");
+    return r != 0 ? r : make_map(&tm[1], p->v, 2, dt, p->D, n, p->Hkv, outer, p->v_stride, ma::kBoxCols, box, "v");
+  };
+  CUtensorMap tm[4] = {};
+  cudaError_t e = cudaSuccess;
+  if (plan.pre_items > 0) {
+    if ((rc = cache_ws_maps(p, plan, dt, true, tm)) != 0 || (rc = kv_maps(tm + 1, 128)) != 0) return rc;
+    a.pairs = plan.pre_pairs;
+    a.by_pairs = ma::fast_div(a.pairs);
+    e = ma::launch_fwd_cache_ws(Dk, bf16, true, tm, a, plan.pre_items, plan.pre_parts, st);
+    if (e != cudaSuccess) return fail(MINIATTN_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+    a.key0 = p->shared_len;
+    a.n_ext = plan.pre_parts;
   }
-  const cudaError_t e = ma::launch_fwd_cache(kernel_head_dim(p->D), p->dtype == MINIATTN_BF16, tm, a, plan.rg, plan.n_ctas,
-                                             reinterpret_cast<cudaStream_t>(stream));
+  if (plan.rg != 0) {
+    if ((rc = kv_maps(tm, 64)) != 0) return rc;
+    e = ma::launch_fwd_cache(Dk, bf16, tm, a, plan.rg, plan.n_ctas, st);
+  } else {
+    if ((rc = cache_ws_maps(p, plan, dt, p->cu_q != nullptr, tm)) != 0 || (rc = kv_maps(tm + 1, 128)) != 0) return rc;
+    a.pairs = plan.pairs;
+    a.by_pairs = ma::fast_div(a.pairs);
+    e = ma::launch_fwd_cache_ws(Dk, bf16, false, tm, a, plan.items, plan.parts, st);
+  }
   if (e != cudaSuccess) return fail(MINIATTN_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   return MINIATTN_OK;
 }

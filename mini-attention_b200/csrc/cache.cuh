@@ -25,9 +25,13 @@ struct CacheArgs {
   int page_shift, n_pages, table_width;  // page size 1 << page_shift
   int window, sinks;       // window 0: none
   int key0;                // keys before it are another launch's (a shared prefix)
-  int n_parts_max;         // CTAs that may share an item (fwd_cache_ws.cu)
   float scale_log2;
-  FastDiv by_g, by_hkv, by_nq;
+  FastDiv by_g, by_nq;
+  // fwd_cache_ws.cu: query heads that share a Q tile (all G of a KV head, or 1), tokens of each in it, pairs of Q tiles per
+  // sequence (ragged: at most), groups of `pack` heads, tiles that a piece of an item has at least
+  int pack, tpt, pairs, groups, min_tiles;
+  FastDiv by_pack, by_pairs, by_groups, by_gqa;
+  int shared;              // a launch over a shared prefix: its tokens
   // scratch: pieces of cut items, un-normalised
   float* part_o;
   float2* part_ml;         // (row maximum in log2 units, row sum)
@@ -103,9 +107,14 @@ __host__ __device__ inline CacheTiles cache_tiles(int lo, int hi, int sink_end) 
   return t;
 }
 
+// Whether [k, k + n) holds keys that no row sees.
+__host__ __device__ inline bool cache_partly_seen(int lo, int hi, int sink_end, int k, int n) {
+  return k + n > hi || (k < lo && k + n > sink_end);
+}
+
 // Whether some row sees one of the keys [k, k + n).
 __host__ __device__ inline bool cache_seen(int lo, int hi, int sink_end, int k, int n) {
-  return k < hi && (k + n > lo || k < sink_end);
+  return k < hi && ((k + n > lo && lo < hi) || k < sink_end);
 }
 
 }  // namespace ma
