@@ -49,6 +49,7 @@ cudaError_t launch_fwd_cache(int D, bool bf16, const CUtensorMap* tm, const Cach
                              cudaStream_t st);
 cudaError_t launch_fwd_cache_ws(int D, bool bf16, bool prefix, const CUtensorMap* tm, const CacheArgs& a, int items, int parts,
                                 cudaStream_t st);
+cudaError_t launch_cache_merge(int D, bool bf16, const CacheArgs& a, int items, int parts, cudaStream_t st);
 cudaError_t launch_append(bool bf16, const AppendArgs& a, int sms, cudaStream_t st);
 cudaError_t launch_wait_selftest(int32_t* status, unsigned long long limit_ns, cudaStream_t st);
 cudaError_t launch_merge_partials(float* acc_o, float* acc_lse, const void* part_o,
@@ -1032,18 +1033,20 @@ struct CachePlan {
   // rows of all sequences: fwd_cache.cu with rg groups of 16 rows, or (rg = 0) fwd_cache_ws.cu in `items` x `parts` CTAs
   int rg, n_ctas;
   int items, parts, pairs;
-  // a launch over the shared prefix before it: items x pieces of each
+  // a launch over the shared prefix before it and one after it that adds its pieces (pre_items = 0: none)
   int pre_items, pre_parts, pre_pairs;
   int pack, tpt, groups;
-  size_t part_rows, ext_rows;
+  size_t part_rows, pre_rows, rest_rows;
   size_t bytes(int D) const {
     const size_t row = kernel_head_dim(D) * sizeof(float);
-    return kCounterBytes + align256(part_rows * sizeof(float2)) + align256(part_rows * row) +
-           align256(ext_rows * sizeof(float2)) + ext_rows * row;
+    size_t n = kCounterBytes;
+    for (size_t rows : {part_rows, pre_rows, rest_rows}) n += align256(rows * sizeof(float2)) + align256(rows * row);
+    return n;
   }
 };
 
-constexpr int kMinPieceTiles = 4;  // 128-key tiles of a piece
+constexpr int kMinPieceTiles = 4;      // 128-key tiles of a piece
+constexpr int kMinPrefixTiles = 2;     // of a shared prefix's, whose pieces a launch of its own adds up
 constexpr long long kMaxPieces = 480;  // of all items together: 64 MB of scratch at D = 128
 
 // Pieces that items of at most `tiles` tiles are cut into.  A CTA takes its tiles and about 4 steps of a tile's time beside
@@ -1078,13 +1081,14 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
     c.n_ctas = 2 * sms;
     c.part_rows = static_cast<size_t>(2 * c.n_ctas) * 16 * c.rg;
     const bool stacked = ragged || p->Nq == 1 || p->q_stride[0] == p->Nq * p->q_stride[2];
-    if (p->shared_len > 0 && stacked) {
-      const long long all = ragged ? p->total_q : static_cast<long long>(p->B) * p->Nq;
-      c.pre_pairs = static_cast<int>((all + span - 1) / span);
+    const long long all = ragged ? p->total_q : static_cast<long long>(p->B) * p->Nq, pairs = (all + span - 1) / span;
+    if (p->shared_len > 0 && p->n_pages > 0 && stacked && pairs * c.groups <= kMaxPieces) {
+      c.pre_pairs = static_cast<int>(pairs);
       c.pre_items = c.pre_pairs * c.groups;
       const int tiles = tiles_of(p->shared_len);
-      c.pre_parts = std::max(1, std::min<int>(sms / std::max(c.pre_items, 1), tiles / kMinPieceTiles));
-      c.ext_rows = static_cast<size_t>(all) * p->Hq * c.pre_parts;
+      c.pre_parts = std::max(1, std::min(sms / c.pre_items, tiles / kMinPrefixTiles));
+      c.pre_rows = static_cast<size_t>(c.pre_items) * c.pre_parts * 2 * ma::kTileM;
+      c.rest_rows = static_cast<size_t>(all) * p->Hq;
     }
     return c;
   }
@@ -1173,10 +1177,19 @@ int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scrat
   const int Dk = kernel_head_dim(p->D);
   uint8_t* at = static_cast<uint8_t*>(scratch);
   a.counters = reinterpret_cast<int*>(at);
-  a.part_ml = reinterpret_cast<float2*>(at += kCounterBytes);
-  a.part_o = reinterpret_cast<float*>(at += align256(plan.part_rows * sizeof(float2)));
-  a.ext_ml = reinterpret_cast<float2*>(at += align256(plan.part_rows * Dk * sizeof(float)));
-  a.ext_o = reinterpret_cast<float*>(at += align256(plan.ext_rows * sizeof(float2)));
+  at += kCounterBytes;
+  const auto take = [&](size_t rows, float2** ml, float** o) {
+    *ml = reinterpret_cast<float2*>(at);
+    *o = reinterpret_cast<float*>(at += align256(rows * sizeof(float2)));
+    at += align256(rows * Dk * sizeof(float));
+  };
+  float2 *part_ml, *pre_ml, *rest_ml;
+  float *part_o, *pre_o, *rest_o;
+  take(plan.part_rows, &part_ml, &part_o);
+  take(plan.pre_rows, &pre_ml, &pre_o);
+  take(plan.rest_rows, &rest_ml, &rest_o);
+  a.part_ml = part_ml;
+  a.part_o = part_o;
   a.pack = plan.pack;
   a.tpt = plan.tpt;
   a.groups = plan.groups;
@@ -1198,23 +1211,36 @@ int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scrat
   };
   CUtensorMap tm[4] = {};
   cudaError_t e = cudaSuccess;
+  const auto pairs_of = [&](int pairs) {
+    a.pairs = pairs;
+    a.by_pairs = ma::fast_div(pairs > 0 ? pairs : 1);
+  };
   if (plan.pre_items > 0) {
     if ((rc = cache_ws_maps(p, plan, dt, true, tm)) != 0 || (rc = kv_maps(tm + 1, 128)) != 0) return rc;
-    a.pairs = plan.pre_pairs;
-    a.by_pairs = ma::fast_div(a.pairs);
+    pairs_of(plan.pre_pairs);
+    a.part_ml = pre_ml;
+    a.part_o = pre_o;
+    a.min_tiles = 1;
     e = ma::launch_fwd_cache_ws(Dk, bf16, true, tm, a, plan.pre_items, plan.pre_parts, st);
     if (e != cudaSuccess) return fail(MINIATTN_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+    a.part_ml = part_ml;
+    a.part_o = part_o;
+    a.rest_ml = rest_ml;
+    a.rest_o = rest_o;
     a.key0 = p->shared_len;
-    a.n_ext = plan.pre_parts;
   }
   if (plan.rg != 0) {
     if ((rc = kv_maps(tm, 64)) != 0) return rc;
     e = ma::launch_fwd_cache(Dk, bf16, tm, a, plan.rg, plan.n_ctas, st);
   } else {
     if ((rc = cache_ws_maps(p, plan, dt, p->cu_q != nullptr, tm)) != 0 || (rc = kv_maps(tm + 1, 128)) != 0) return rc;
-    a.pairs = plan.pairs;
-    a.by_pairs = ma::fast_div(a.pairs);
+    pairs_of(plan.pairs);
     e = ma::launch_fwd_cache_ws(Dk, bf16, false, tm, a, plan.items, plan.parts, st);
+  }
+  if (e == cudaSuccess && plan.pre_items > 0) {
+    a.part_ml = pre_ml;
+    a.part_o = pre_o;
+    e = ma::launch_cache_merge(Dk, bf16, a, plan.pre_items, plan.pre_parts, st);
   }
   if (e != cudaSuccess) return fail(MINIATTN_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   return MINIATTN_OK;

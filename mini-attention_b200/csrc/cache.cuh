@@ -27,8 +27,8 @@ struct CacheArgs {
   int key0;                // keys before it are another launch's (a shared prefix)
   float scale_log2;
   FastDiv by_g, by_nq;
-  // fwd_cache_ws.cu: query heads that share a Q tile (all G of a KV head, or 1), tokens of each in it, pairs of Q tiles per
-  // sequence (ragged: at most), groups of `pack` heads, tiles that a piece of an item has at least
+  // fwd_cache_ws.cu: query heads that share a Q tile (all G of a KV head, or 1), tokens of each in it, pairs of Q tiles of a
+  // sequence (not ragged), groups of `pack` heads, tiles that a piece of an item has at least
   int pack, tpt, pairs, groups, min_tiles;
   FastDiv by_pack, by_pairs, by_groups, by_gqa;
   int shared;              // a launch over a shared prefix: its tokens
@@ -36,11 +36,21 @@ struct CacheArgs {
   float* part_o;
   float2* part_ml;         // (row maximum in log2 units, row sum)
   int* counters;           // zero between launches
-  // pieces of every row that another launch left (a shared prefix): [n_ext][rows of q * Hq][D] and (m, l)
-  const float* ext_o;
-  const float2* ext_ml;
-  int n_ext;
+  // Not null: nothing is written to o; every row's un-normalised O and (m, l) go here, [rows of q * Hq][D] and
+  // [rows of q * Hq], for the launch that adds the shared prefix's pieces.
+  float* rest_o;
+  float2* rest_ml;
 };
+
+// x / y, neither negative.  Not inlined on the device: a kernel's start is bound by the code it fetches for the first time.
+#ifdef __CUDACC__
+static __host__ __device__ __noinline__ long long cache_div(long long x, long long y) {
+#else
+inline long long cache_div(long long x, long long y) {
+#endif
+  if (((x | y) >> 31) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
+}
 
 // One sequence of a call.  Keys that some row of it sees: [lo, hi) and, with a window, [0, sink_end) before them.
 struct CacheSeq {

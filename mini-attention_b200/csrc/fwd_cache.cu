@@ -12,7 +12,7 @@
 //   warps 0-3 16 rows x (16 * RG keys of the tile) each, running (m, l, O) in registers
 //
 // A CTA whose range cuts an item leaves its piece (un-normalised O, m, l) in scratch and counts itself in; the one that
-// counts in last folds the pieces, those that another launch left for these rows among them (a shared prefix).
+// counts in last folds the pieces.  Behind a shared prefix the rows are left un-normalised for the launch that adds its pieces.
 //
 // Keys that no row sees are never read: their pages may be gone or hold anything.  Where a tile holds some, their scores
 // are replaced and their rows of V cleared, so that what lies there does not reach a result.
@@ -32,6 +32,7 @@ constexpr int kKeys = 64;            // keys per tile
 constexpr int kBox = kKeys * 128;    // one [64 keys x 128 B] box
 constexpr float kLazy = 8.0f;        // log2 units a row's maximum may move before O is rescaled
 constexpr int kMergePitch = 36;      // floats per row of the merge buffer (32 + padding)
+constexpr int kPiece = 8;            // tiles of a piece where every CTA works on one
 
 template <int D>
 struct Layout {
@@ -41,8 +42,8 @@ struct Layout {
   static constexpr int kOffMerge = kStages * kStageBytes;              // float[4 warps][16][kMergePitch]
   static constexpr int kOffMl = kOffMerge + 4 * 16 * kMergePitch * 4;  // float2[4 warps][16]
   static constexpr int kOffBar = kOffMl + 4 * 16 * 8;                  // full[kStages], empty[kStages]
-  static constexpr int kOffScan = kOffBar + 2 * kStages * 8;           // long long[4 warps], start, total
-  static constexpr int kOffMisc = kOffScan + 6 * 8;                    // abort flag, arrival order, first sequence
+  static constexpr int kOffScan = kOffBar + 2 * kStages * 8;           // long long[2][4 warps], tiles before the first sequence
+  static constexpr int kOffMisc = kOffScan + 10 * 8;                   // abort flag, arrival order, first sequence
   static constexpr int kBytes = kOffMisc + 16;
   static constexpr int kDynSmem = kBytes + 1024;
 };
@@ -75,17 +76,18 @@ __device__ __forceinline__ float row_lse(float m, float l) {
   return l == 0.f ? -INFINITY : m * 0.6931471805599453f + __logf(l);
 }
 
-// Sequence b of the call, and how its items are counted: n_rb row blocks per KV head, tiles of each.
+// Sequence b of the call, and how its items are counted: n_rb row blocks per KV head, `slots` places of the launch's tiles
+// for each (its t.n tiles and, where a launch is so short that a CTA works on one piece, what fills the last piece up).
 struct Walk {
   CacheSeq s;
   CacheTiles t;
-  int n_rb;
+  int n_rb, slots;
   __device__ __forceinline__ long long total(const CacheArgs& a) const {
-    return static_cast<long long>(a.Hkv) * n_rb * t.n;
+    return static_cast<long long>(a.Hkv) * n_rb * slots;
   }
 };
 template <int kRows>
-__device__ __forceinline__ Walk walk_to(const CacheArgs& a, int b) {
+__device__ __forceinline__ Walk walk_to(const CacheArgs& a, int b, bool pieces) {
   Walk w;
   int r0 = 0, r1 = 0;
   if (a.cu_q != nullptr) {
@@ -95,6 +97,7 @@ __device__ __forceinline__ Walk walk_to(const CacheArgs& a, int b) {
   w.s = cache_seq(a, r0, r1, a.seq_lens != nullptr ? a.seq_lens[b] : 0);
   w.t = cache_tiles<kKeys>(w.s.lo, w.s.hi, w.s.sink_end);
   w.n_rb = static_cast<int>((static_cast<long long>(w.s.nq) * a.G + kRows - 1) / kRows);
+  w.slots = pieces ? (w.t.n + (kPiece - 1)) / kPiece * kPiece : w.t.n;
   return w;
 }
 
@@ -102,8 +105,7 @@ __device__ __forceinline__ Walk walk_to(const CacheArgs& a, int b) {
 
 template <int D, bool BF16, int RG>
 __global__ void __launch_bounds__(kThreads, 2)
-fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a,
-                 int min_share) {
+fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a) {
   using L = Layout<D>;
   constexpr int KG = 4 / RG;      // key groups: warps that share a row group
   constexpr int kRows = 16 * RG;  // rows of an item
@@ -136,54 +138,74 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   }
   grid_dep_wait();
 
-  // ---- this CTA's tiles [lo, hi) of the launch's total: each of 128 threads adds up a run of sequences ----
+  // ---- this CTA's tiles [lo, hi) of the launch's total: each of 128 threads adds up a run of sequences.  Where pieces of
+  // kPiece tiles, none with tiles of two items, are no more than the CTAs, each CTA takes one; otherwise all tiles are cut
+  // alike. ----
   const int run = (a.B + 127) / 128;
   const int b0 = min(a.B, tid * run), b1 = tid < 128 ? min(a.B, b0 + run) : b0;
-  long long mine = 0;
+  long long mine = 0, mine_pieces = 0;
   bool bad = false;
   for (int b = b0; b < b1; ++b) {
-    const Walk w = walk_to<kRows>(a, b);
-    mine += w.total(a);
+    const Walk w = walk_to<kRows>(a, b, true);
+    const long long items = static_cast<long long>(a.Hkv) * w.n_rb;
+    mine += items * w.t.n;
+    mine_pieces += items * w.slots;
     bad |= w.s.bad;
   }
   if (bad && a.status != nullptr) atomicOr(a.status, kErrCache);
-  long long before = mine;  // inclusive over the warp, then exclusive over the CTA
+  long long before = mine, before_pieces = mine_pieces;  // inclusive over the warp, then exclusive over the CTA
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, before, d);
-    if (lane >= d) before += o;
+    const long long o = __shfl_up_sync(0xffffffffu, before, d), op = __shfl_up_sync(0xffffffffu, before_pieces, d);
+    if (lane >= d) {
+      before += o;
+      before_pieces += op;
+    }
   }
-  if (lane == 31 && warp < 4) scan[warp] = before;
+  if (lane == 31 && warp < 4) {
+    scan[warp] = before;
+    scan[4 + warp] = before_pieces;
+  }
   __syncthreads();
-  long long total = 0;
+  long long total = 0, total_pieces = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    if (w < warp) before += scan[w];
+    if (w < warp) {
+      before += scan[w];
+      before_pieces += scan[4 + w];
+    }
     total += scan[w];
+    total_pieces += scan[4 + w];
+  }
+  const long long n_ctas = gridDim.x;
+  const bool pieces = total_pieces <= n_ctas * kPiece;
+  const long long share = pieces ? kPiece : cache_div(total + n_ctas - 1, n_ctas);
+  if (pieces) {
+    total = total_pieces;
+    before = before_pieces;
+    mine = mine_pieces;
   }
   before -= mine;
-  const long long n_ctas = gridDim.x;
-  const long long share = max(static_cast<long long>(min_share), (total + n_ctas - 1) / n_ctas);
   const long long lo = blockIdx.x * share, hi = min(total, lo + share);
   if (lo >= hi) return;
   if (tid < 128 && lo >= before && lo < before + mine) {
     int b = b0;
     for (;; ++b) {
-      const long long n = walk_to<kRows>(a, b).total(a);
+      const long long n = walk_to<kRows>(a, b, pieces).total(a);
       if (lo < before + n) break;
       before += n;
     }
     *first_seq = b;
-    scan[4] = before;
+    scan[8] = before;
   }
   __syncthreads();
   int b = *first_seq;
-  long long base = scan[4];  // tiles before sequence b
-  Walk w = walk_to<kRows>(a, b);
+  long long base = scan[8];  // tiles before sequence b
+  Walk w = walk_to<kRows>(a, b, pieces);
   auto next_seq = [&]() {  // the next sequence that has rows; only while tiles are left
     do {
       base += w.total(a);
-      w = walk_to<kRows>(a, ++b);
+      w = walk_to<kRows>(a, ++b, pieces);
     } while (w.n_rb == 0);
   };
 
@@ -198,14 +220,9 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const uint32_t dst = (is_v ? L::kBoxes * kBox : 0) + bx * kBox + ((sub << keys_shift) << 7);
     const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
     const uint32_t box_bytes = 128u << keys_shift;
-    int hk, j;
-    auto locate = [&](long long x) {
-      const long long within = x - base, it = within / w.t.n;
-      j = static_cast<int>(within - it * w.t.n);
-      hk = static_cast<int>(it / w.n_rb);
-      return static_cast<int>(it - static_cast<long long>(hk) * w.n_rb);
-    };
-    int rb = locate(lo);
+    const long long it0 = cache_div(lo - base, w.slots);
+    int j = static_cast<int>(lo - base - it0 * w.slots);
+    int hk = static_cast<int>(cache_div(it0, w.n_rb)), rb = static_cast<int>(it0 - static_cast<long long>(hk) * w.n_rb);
     int key = 0, page = 0;
     bool wanted = false;
     auto look_up = [&]() {  // the page of this lane's keys of tile j
@@ -223,7 +240,9 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     };
     look_up();
     int slot = 0, par = 1, i = 0;
-    for (long long x = lo; x < hi; ++x, ++i) {
+    // with pieces, hi may lie past the item's last tile: the CTA has none after it
+    const int n_mine = static_cast<int>(pieces ? min(hi - lo, static_cast<long long>(w.t.n - j)) : hi - lo);
+    for (; i < n_mine; ++i) {
       if (i >= L::kStages) mbar_wait(empty(slot), par, wc, kErrWaitFree);
       const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, wanted));
       if (lane == 0) mbar_expect_tx(full(slot), n_copies * box_bytes);
@@ -234,7 +253,7 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         slot = 0;
         par ^= 1;
       }
-      if (x + 1 < hi) {
+      if (i + 1 < n_mine) {
         if (++j == w.t.n) {
           j = 0;
           if (++rb == w.n_rb) {
@@ -271,11 +290,11 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
   for (long long x = lo; x < hi;) {
     while (x >= base + w.total(a)) next_seq();
-    const long long it = (x - base) / w.t.n;
-    const long long item0 = base + it * w.t.n;
+    const long long it = cache_div(x - base, w.slots);
+    const long long item0 = base + it * w.slots;
     const int t0 = static_cast<int>(x - item0);
     const int t1 = static_cast<int>(min(static_cast<long long>(w.t.n), hi - item0));
-    const int hk = static_cast<int>(it / w.n_rb), rb = static_cast<int>(it - static_cast<long long>(hk) * w.n_rb);
+    const int hk = static_cast<int>(cache_div(it, w.n_rb)), rb = static_cast<int>(it - static_cast<long long>(hk) * w.n_rb);
     const int rows = w.s.nq * a.G, row0 = rb * kRows;
 
     // Q fragments of this warp's 16 rows, and which keys its two rows of this lane see
@@ -434,8 +453,8 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     }
 
     // ---- end of a piece: fold the key groups, then write the rows or publish the partial ----
-    const bool all_tiles = t0 == 0 && t1 == w.t.n;
-    const bool whole = all_tiles && a.n_ext == 0;
+    const bool whole = t0 == 0 && t1 == w.t.n;
+    const bool rest = a.rest_o != nullptr;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
@@ -455,13 +474,17 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         lt += ml.y * part_weight(ml.x, mt);
       }
       f[e] = part_weight(m_run[e], mt);
-      if (whole) f[e] *= lt > 0.f ? 1.f / lt : lt;  // a NaN stays one
+      if (whole && !rest) f[e] *= lt > 0.f ? 1.f / lt : lt;  // a NaN stays one
     }
-    const long long c_first = item0 / share;  // CTA that holds the item's first tile
+    const long long c_first = cache_div(item0, share);  // CTA that holds the item's first tile
     const long long my_slot = 2ll * blockIdx.x + (t0 == 0 ? 1 : 0);
     auto lse_at = [&](int r) -> float* {
       const int tok = div_by(r, a.by_g), h = hk * a.G + (r - tok * a.G);
       return a.lse + b * a.ls[0] + h * a.ls[1] + w.s.row0 + tok;
+    };
+    auto rest_row = [&](int r) -> long long {
+      const int tok = div_by(r, a.by_g), h = hk * a.G + (r - tok * a.G);
+      return ((a.cu_q != nullptr ? w.s.row0 : static_cast<long long>(b) * a.Nq) + tok) * a.Hq + h;
     };
     if (tid < kRows && row0 + tid < rows) {
       const int rgi = tid >> 4, rr = tid & 15;
@@ -472,9 +495,15 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         lt += ml.y * part_weight(ml.x, mt);
       }
       if (!whole) a.part_ml[my_slot * kRows + tid] = make_float2(mt, lt);
+      else if (rest) a.rest_ml[rest_row(row0 + tid)] = make_float2(mt, lt);
       else if (a.lse != nullptr) *lse_at(row0 + tid) = row_lse(mt, lt);
     }
     auto store_row = [&](int r_in, int col, const float4& o) {  // four columns of a finished row
+      if (rest) {
+        *reinterpret_cast<float4*>(a.rest_o + rest_row(row0 + r_in) * D + col) = o;
+        return;
+      }
+      if (col >= a.D) return;
       const int r = row0 + r_in, tok = div_by(r, a.by_g), h = hk * a.G + (r - tok * a.G);
       uint2 y;
       y.x = pack2<BF16>(o.x, o.y);
@@ -509,59 +538,52 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
         const int col = p * 32 + c4;
         if (!whole) *reinterpret_cast<float4*>(a.part_o + (my_slot * kRows + r_in) * D + col) = o;
-        else if (col < a.D) store_row(r_in, col, o);
+        else store_row(r_in, col, o);
       }
       workers_sync();
     }
     if (!whole) {
-      int n_parts = 1;
-      if (!all_tiles) {
-        __threadfence();  // release: the piece before the count
-        workers_sync();
-        n_parts = static_cast<int>((item0 + w.t.n - 1) / share - c_first + 1);
-        if (tid == 0) {
-          __threadfence();
-          *order = atomicAdd(a.counters + c_first, 1);
+      __threadfence();  // release: the piece before the count
+      workers_sync();
+      const int n_parts = static_cast<int>(cache_div(item0 + w.slots - 1, share) - c_first + 1);
+      if (tid == 0) {
+        __threadfence();
+        *order = atomicAdd(a.counters + c_first, 1);
+      }
+      workers_sync();
+      if (*order == n_parts - 1) {
+        __threadfence();  // acquire: every other piece was published before it was counted
+        if (tid == 0) a.counters[c_first] = 0;
+        const int n_rows = min(kRows, rows - row0);
+        // where the pieces of a row lie: the first, the others two slots apart
+        auto piece = [&](int p, int r_in) { return (2 * (c_first + p) + (p == 0 ? 1 : 0)) * kRows + r_in; };
+        // total maximum of every row: 128 / kRows threads share a row
+        constexpr int kPerRow = 128 / kRows;
+        {
+          const int r_in = tid / kPerRow;
+          float m = -INFINITY;
+          if (r_in < n_rows) {
+#pragma unroll 4
+            for (int p = tid % kPerRow; p < n_parts; p += kPerRow) m = fmaxf(m, __ldcg(a.part_ml + piece(p, r_in)).x);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int d = kPerRow / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+          if (tid % kPerRow == 0) merge[r_in] = m;
         }
         workers_sync();
-      } else {
-        __threadfence();  // the CTA reads its own piece back
-        workers_sync();
-      }
-      if (all_tiles || *order == n_parts - 1) {
-        __threadfence();  // acquire: every other piece was published before it was counted
-        if (!all_tiles && tid == 0) a.counters[c_first] = 0;
-        const int n_rows = min(kRows, rows - row0), n_all = n_parts + a.n_ext;
-        const long long ext_rows = (a.cu_q != nullptr ? a.total_q : static_cast<long long>(a.B) * a.Nq) * a.Hq;
-        // where piece p of a row lies: its own launch's pieces, then the other launch's
-        auto piece = [&](int p, int r_in, const float2** ml, const float** o) {
-          if (p < n_parts) {
-            const long long i = (2 * (c_first + p) + (p == 0 ? 1 : 0)) * kRows + r_in;
-            *ml = a.part_ml + i;
-            *o = a.part_o + i * D;
-          } else {
-            const int r = row0 + r_in, tok = div_by(r, a.by_g), h = hk * a.G + (r - tok * a.G);
-            const long long q_row = a.cu_q != nullptr ? w.s.row0 + tok : static_cast<long long>(b) * a.Nq + tok;
-            const long long i = (p - n_parts) * ext_rows + q_row * a.Hq + h;
-            *ml = a.ext_ml + i;
-            *o = a.ext_o + i * D;
-          }
-        };
+        // four columns of a row per thread, the loads of eight pieces in flight together
         const int n_el = n_rows * (D / 4);
         for (int e = tid; e < n_el; e += 128) {
           const int r_in = e / (D / 4), col = (e % (D / 4)) * 4;
-          const float2* ml;
-          const float* po;
-          float mt = -INFINITY, lt = 0.f;
-          for (int p = 0; p < n_all; ++p) {
-            piece(p, r_in, &ml, &po);
-            mt = fmaxf(mt, __ldcg(ml).x);
-          }
+          const float mt = merge[r_in];
+          float lt = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int p = 0; p < n_all; ++p) {
-            piece(p, r_in, &ml, &po);
-            const float2 x2 = __ldcg(ml);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(po + col));
+#pragma unroll 8
+          for (int p = 0; p < n_parts; ++p) {
+            const long long i = piece(p, r_in);
+            const float2 x2 = __ldcg(a.part_ml + i);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_o + i * D + col));
             const float wgt = part_weight(x2.x, mt);
             lt = fmaf(x2.y, wgt, lt);
             o.x = fmaf(y.x, wgt, o.x);
@@ -569,18 +591,21 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             o.z = fmaf(y.z, wgt, o.z);
             o.w = fmaf(y.w, wgt, o.w);
           }
-          const float inv = lt > 0.f ? 1.f / lt : lt;
+          const float inv = rest ? 1.f : lt > 0.f ? 1.f / lt : lt;
           o.x *= inv;
           o.y *= inv;
           o.z *= inv;
           o.w *= inv;
-          if (col < a.D) store_row(r_in, col, o);
-          if (col == 0 && a.lse != nullptr) *lse_at(row0 + r_in) = row_lse(mt, lt);
+          store_row(r_in, col, o);
+          if (col == 0) {
+            if (rest) a.rest_ml[rest_row(row0 + r_in)] = make_float2(mt, lt);
+            else if (a.lse != nullptr) *lse_at(row0 + r_in) = row_lse(mt, lt);
+          }
         }
       }
       workers_sync();  // `order` may be written again only when everyone has read it
     }
-    x = item0 + t1;
+    x = item0 + (t1 == w.t.n ? w.slots : t1);
   }
 }
 
@@ -591,7 +616,7 @@ static cudaError_t launch_t(const CUtensorMap* tm, const CacheArgs& a, int n_cta
   static std::atomic<unsigned long long> smem_set{0};
   cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kern), Layout<D>::kDynSmem, &smem_set);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(kern, n_ctas, kThreads, Layout<D>::kDynSmem, st, tm[0], tm[1], a, 4);
+  return launch_overlapped(kern, n_ctas, kThreads, Layout<D>::kDynSmem, st, tm[0], tm[1], a);
 }
 
 template <int D, bool BF16>

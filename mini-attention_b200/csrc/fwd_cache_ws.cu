@@ -4,15 +4,15 @@
 //   item      = two 128-row Q tiles of one sequence and one KV head; the `pack` query heads of the KV head share them, row r of
 //               a tile is token r / pack, head r % pack
 //   warps 0-3 softmax of Q tile 0 (thread = row), its epilogue; warps 4-7 the same for Q tile 1
-//   warp 8    MMA issuer of Q tile 0, warp 10 of Q tile 1; warp 9 TMA producer; warp 11 zeroes padding rows of the Q tiles
+//   warp 8    MMA issuer of Q tile 0, warp 10 of Q tile 1
+//   warp 9    finds the item, copies Q and K; warp 11 copies V (and zeroes padding rows of the Q tiles before that)
 //
 // An item visits the 128-key tiles that its rows see: those of the sinks, then those from the window of its first row to its
 // last row's position, each as two 64-key halves.  Where there are few items their tiles are cut into pieces: every piece
 // leaves (un-normalised O, m, l) in scratch and counts itself in, and the one that counts in last folds them, in their order.
 //
 // Tiles at the ends hold keys that no row of the sequence sees and that may be anything.  Their scores are replaced; their
-// rows of V are cleared in shared memory by the producer, which hands such a tile over itself instead of leaving that to the
-// copy.
+// rows of V are cleared in shared memory by warp 11, which hands such a tile over itself instead of leaving that to the copy.
 #include <atomic>
 
 #include "cache.cuh"
@@ -24,7 +24,7 @@ namespace ma {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10, kWarpIdle = 11;
+constexpr int kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10, kWarpV = 11;
 constexpr int kHalfN = kTileN / 2;   // keys per half tile
 constexpr float kSumLimit = 256.0f;  // a half's sum of P above which the row's reference moves
 // registers per thread after setmaxnreg: 8 * 216 + 4 * 72 = 12 * 168, what the launch allocates
@@ -47,7 +47,7 @@ struct Layout {
   static constexpr int kBarPReady = kBarSFull + 4;          // [2][2] softmax -> MMA
   static constexpr int kBarODone = kBarPReady + 4;          // [2][2] MMA -> softmax (rescale, epilogue)
   static constexpr int kBarStagger = kBarODone + 4;         // one-shot: tile 0 published its first row maxima
-  static constexpr int kBarRaw = kBarStagger + 1;           // copy of a V tile that the producer hands over itself
+  static constexpr int kBarRaw = kBarStagger + 1;           // copy of a V tile that warp 11 hands over itself
   static constexpr int kNumBars = kBarRaw + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;   // tmem slot, abort flag, arrival order [2]
   static constexpr int kOffItem = kOffMisc + 32;            // WsItem
@@ -84,8 +84,54 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 __device__ __forceinline__ float part_weight(float m, float mt) { return m == -INFINITY ? 0.f : ex2(m - mt); }
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.f ? -INFINITY : m * 0.6931471805599453f + __logf(l);
+}
 // bits [0, x) of 64
 __device__ __forceinline__ uint64_t below(int x) { return x <= 0 ? 0ull : x >= 64 ? ~0ull : (1ull << x) - 1; }
+
+// What a lane copies of a 128-key tile: 64 columns of the keys of one page.  Pages are fetched a tile ahead, since the ring has
+// no room for the time that takes.
+template <int kBoxes>
+struct PageLane {
+  int shift, sub, bx;  // keys of a box (1 << shift: a page's, at most 128), the lane's among the tile's, its columns
+  int page = 0, key = 0, next_page = 0, next_key = 0;
+  bool wanted = false, next_wanted = false;
+  __device__ __forceinline__ PageLane(const CacheArgs& a)
+      : shift(a.table != nullptr ? min(7, a.page_shift) : 7), sub((threadIdx.x & 31) / kBoxes), bx((threadIdx.x & 31) % kBoxes) {}
+  __device__ __forceinline__ void fetch(const CacheArgs& a, const WsItem& it, int j) {  // tile number j of the item
+    next_key = it.t.at(j) * kTileN + (sub << shift);
+    next_wanted = sub < (kTileN >> shift) && cache_seen(it.s.lo, it.s.hi, it.s.sink_end, next_key, 1 << shift);
+    next_page = it.b;
+    if (a.table != nullptr && next_wanted) next_page = a.table[it.b * a.table_stride + (next_key >> a.page_shift)];
+  }
+  __device__ __forceinline__ void settle(const CacheArgs& a) {
+    page = next_page;
+    key = next_key;
+    wanted = next_wanted;
+    if (a.table != nullptr) {
+      key &= (1 << a.page_shift) - 1;
+      if (wanted && static_cast<unsigned>(page) >= static_cast<unsigned>(a.n_pages)) {
+        wanted = false;
+        if (a.status != nullptr) atomicOr(a.status, kErrCache);
+      }
+    }
+  }
+  __device__ __forceinline__ void copy(const CUtensorMap* tm, uint32_t dst, uint32_t full, int hk) const {  // the whole warp
+    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, wanted)) * (128u << shift);
+    if ((threadIdx.x & 31) == 0) mbar_expect_tx(full, bytes);
+    __syncwarp();
+    if (wanted) tma_load_4d(dst + bx * kBoxBytes + ((sub << shift) << 7), tm, full, bx * kBoxCols, key, hk, page);
+    __syncwarp();
+  }
+};
+
+// Give-up path: copies may still be in flight; let them land (bounded) before the shared memory is released.
+__device__ __forceinline__ void wait_for_copies() {
+  const uint64_t t0 = global_timer_ns();
+  while (global_timer_ns() - t0 < 2000000ull) {
+  }
+}
 
 // Sequence and pair of Q tiles of pair number `idx` of a ragged launch; the whole warp.  False: fewer pairs than that.
 __device__ __forceinline__ bool ragged_pair(const CacheArgs& a, int idx, int* b, int* pair, CacheSeq* s) {
@@ -124,7 +170,7 @@ __device__ __forceinline__ bool ragged_pair(const CacheArgs& a, int idx, int* b,
 }  // namespace
 
 // PREFIX: the rows are those of all sequences, one after the other, the keys the a.shared first tokens of sequence 0's block
-// table; every piece is left for the launch that folds it (CacheArgs::ext_o), nothing is written to o.
+// table; every piece is left for cache_merge_kernel, nothing is written to o.
 // NARROW: head dim 96 on the D = 128 tiles, the MMAs leave the 32 columns of zeros out.
 template <int D, bool BF16, bool PREFIX, bool NARROW>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -153,41 +199,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int tpt = a.tpt;
   const WaitCtx wc{abort_flag, a.status, MINIATTN_WAIT_LIMIT_NS};
 
-  // ---- TMA producer: what it copies for fill i of the ring, K (even) or V (odd) of tile number it.j0 + i / 2.  Lane l copies
-  // 64 columns of the keys of one page.
-  const int keys_shift = a.table != nullptr ? min(7, a.page_shift) : 7;  // keys of a box
-  const int sub = lane / L::kBoxes, my_bx = lane % L::kBoxes;
-  int page = 0, key = 0;
-  bool wanted = false;
-  auto look_up = [&](const WsItem& it, int j) {  // this lane's page of tile number j
-    const int k0 = it.t.at(j) * kTileN + (sub << keys_shift);
-    key = k0;
-    wanted = sub < (kTileN >> keys_shift) && cache_seen(it.s.lo, it.s.hi, it.s.sink_end, k0, 1 << keys_shift);
-    page = it.b;
-    if (a.table != nullptr) {
-      key = k0 & ((1 << a.page_shift) - 1);
-      if (wanted) {
-        page = a.table[it.b * a.table_stride + (k0 >> a.page_shift)];
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.n_pages)) {
-          wanted = false;
-          if (a.status != nullptr) atomicOr(a.status, kErrCache);
-        }
-      }
-    }
-  };
-  auto copy_tile = [&](const WsItem& it, int i, uint32_t full) {  // the whole warp
-    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, wanted)) * (128u << keys_shift);
-    if (lane == 0) mbar_expect_tx(full, bytes);
-    __syncwarp();
-    if (wanted)
-      tma_load_4d(sRing + (i % L::kStages) * L::kTileBytes + my_bx * kBoxBytes + ((sub << keys_shift) << 7),
-                  (i & 1) ? &tm_v : &tm_k, full, my_bx * kBoxCols, key, div_by(it.group, a.by_gqa), page);
-    __syncwarp();
-  };
-  auto dirty = [&](const WsItem& it, int j) {
-    return cache_partly_seen(it.s.lo, it.s.hi, it.s.sink_end, it.t.at(j) * kTileN, kTileN);
-  };
-  int next_fill = 0;  // producer warp: fills that have been issued
+  PageLane<L::kBoxes> pl(a);  // warps 9 and 11
 
   if (warp == kWarpTma) {
     for (int i = lane; i < L::kNumBars; i += 32) {
@@ -264,14 +276,10 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
       }
       __syncwarp();
-      look_up(it, it.j0);
-      while (next_fill < min(2 * it.n, L::kStages)) {
-        const int i = next_fill;
-        if ((i & 1) && dirty(it, it.j0 + (i >> 1))) break;  // handed over below
-        copy_tile(it, i, bar(L::kBarKvFull + i % L::kStages));
-        ++next_fill;
-        if ((i & 1) && next_fill < 2 * it.n) look_up(it, it.j0 + (next_fill >> 1));
-      }
+      pl.fetch(a, it, it.j0);
+      pl.settle(a);
+      if (it.n > 1) pl.fetch(a, it, it.j0 + 1);
+      pl.copy(&tm_k, sRing, bar(L::kBarKvFull), div_by(it.group, a.by_gqa));
     }
   }
   if (warp == kWarpMma0) {
@@ -281,7 +289,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   {
     // where pack does not divide 128 the last rows of the Q tiles belong to nobody; zeros keep their scores finite
     const int pad = kTileM - a.pack * tpt;
-    if (warp == kWarpIdle && pad > 0) {
+    if (warp == kWarpV && pad > 0) {
       for (int i = lane; i < 2 * L::kBoxes * pad * 8; i += 32) {
         const int box = i / (pad * 8), at = i % (pad * 8);
         *reinterpret_cast<uint4*>(gbase + L::kOffQ + box * kBoxBytes + (kTileM - pad) * 128 + at * 16) =
@@ -316,7 +324,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       int first, end;
       if constexpr (PREFIX) {
         first = 0;
-        end = 0;
+        end = it.s.hi;
         if (real) {
           int b, i, r0 = 0, r1 = 0;
           if (a.cu_q != nullptr) {
@@ -344,8 +352,11 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
         __syncwarp();
       } else {
-        cache_row(a, it.s, tok, &first, &end);
+        // rows that are nobody's see what their tile's last one does
+        cache_row(a, it.s, min(it.q0 + t * tpt + min(in_tile, tpt - 1), it.s.nq - 1), &first, &end);
       }
+      // what all rows of the warp see, so that the tiles in between need no look at their keys
+      const int all_from = __reduce_max_sync(0xffffffffu, first), all_to = __reduce_min_sync(0xffffffffu, end);
       float m_cur = -INFINITY;  // running (lazily updated) row maximum, log2 units
       float l_run = 0.f;
 
@@ -361,10 +372,12 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           tmem_ld32(tS + hb * kHalfN + 32, s[1]);
           tmem_wait_ld();
           const int k0 = k_tile + hb * kHalfN;
-          if (end - k0 < kHalfN || first > k0) {
+          bool sees = true;  // this row, some key of this half
+          if (k0 < all_from || k0 + kHalfN > all_to) {
             // by selection: what a hidden key's score holds does not matter
             const uint64_t seen = below(end - k0) & (~below(first - k0) | below(a.sinks - k0));
             const uint32_t part[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
+            sees = seen != 0;
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -437,7 +450,8 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 pk[q * 16 + (i >> 1)] = pack2<BF16>(p0, p1);
               }
             unpack_f32x2(psum, psum0, psum1);
-            if (pass == 1 || !__any_sync(0xffffffffu, !(psum0 + psum1 <= kSumLimit) || m_cur == -INFINITY)) break;
+            // again where the sum is too large, or the row sees its first keys
+            if (pass == 1 || !__any_sync(0xffffffffu, !(psum0 + psum1 <= kSumLimit) || (m_cur == -INFINITY && sees))) break;
             fix = true;
           }
           l_run += psum0 + psum1;
@@ -464,28 +478,9 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       };
       bool write_out = !PREFIX;
       float m_tot = m_cur, l_tot = l_run;
-      if constexpr (PREFIX) {
-        // every lane takes part in the reads of TMEM; rows that are nobody's store nothing
-        const long long rows = static_cast<long long>(it.s.nq) * a.Hq;
-        const long long at = it.part * rows + static_cast<long long>(tok) * a.Hq + head;
-        if (real) const_cast<float2*>(a.ext_ml)[at] = make_float2(m_cur, l_run);
-        float4* po = reinterpret_cast<float4*>(const_cast<float*>(a.ext_o) + at * D);
-#pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32] = {};
-          if (q < kCols / 32) chunk(q, o);
-          if (real) {
-#pragma unroll
-            for (int g = 0; g < 8; ++g)
-              po[q * 8 + g] = make_float4(__uint_as_float(o[4 * g]), __uint_as_float(o[4 * g + 1]),
-                                          __uint_as_float(o[4 * g + 2]), __uint_as_float(o[4 * g + 3]));
-          }
-          __syncwarp();
-        }
-      }
       // slots of the item's pieces: [piece][tile][D / 4][128 rows][4] floats, a warp stores 512 bytes in a row
       const long long slot0 = static_cast<long long>(it.item) * gridDim.y * 2 + t;
-      if (!PREFIX && it.n_parts > 1) {
+      if (PREFIX || it.n_parts > 1) {
         const long long my = (slot0 + 2 * it.part) * kTileM;
         a.part_ml[my + r] = make_float2(m_cur, l_run);
         float4* po = reinterpret_cast<float4*>(a.part_o + my * D) + r;
@@ -498,6 +493,8 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             po[(q * 8 + g) * kTileM] = make_float4(__uint_as_float(o[4 * g]), __uint_as_float(o[4 * g + 1]),
                                                    __uint_as_float(o[4 * g + 2]), __uint_as_float(o[4 * g + 3]));
         }
+      }
+      if (!PREFIX && it.n_parts > 1) {
         __threadfence();  // release: the piece before the count
         named_bar_sync(1 + t, 128);
         if (r == 0) {
@@ -679,21 +676,27 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
       }
       __syncwarp();
-    } else if (warp == kWarpTma && nt > 0 && n_tiles > 0) {
-      // =========================== TMA producer ====================================
+    } else if (nt > 0 && n_tiles > 0) {
+      // =========================== copies ==========================================
+      // Fill i of the ring is K (even) or V (odd) of tile i / 2: warp 9 takes the even ones, warp 11 the odd ones.
+      const bool is_v = warp == kWarpV;
       uint32_t raw_phase = 0;
-      for (int i = next_fill; i < 2 * n_tiles; ++i) {
-        const int slot = i % L::kStages, j = it.j0 + (i >> 1);
+      const int hk = div_by(it.group, a.by_gqa);
+      if (is_v) pl.fetch(a, it, it.j0);
+      for (int j = is_v ? 0 : 1; j < n_tiles; ++j) {
+        const int i = 2 * j + (is_v ? 1 : 0), slot = i % L::kStages, k0 = it.t.at(it.j0 + j) * kTileN;
+        pl.settle(a);
+        if (j + 1 < n_tiles) pl.fetch(a, it, it.j0 + j + 1);
         if (i >= L::kStages) {
           __nanosleep(200);  // a sleeping warp takes no issue slots from the softmax warps beside it
           mbar_wait(bar(L::kBarKvEmpty + slot), (i / L::kStages - 1) & 1, wc, kErrWaitFree);
         }
-        const uint32_t full = bar(L::kBarKvFull + slot);
-        if ((i & 1) && dirty(it, j)) {
-          copy_tile(it, i, bar(L::kBarRaw));
-          mbar_wait(bar(L::kBarRaw), raw_phase, wc, kErrWaitKV);
+        const bool clear = is_v && cache_partly_seen(it.s.lo, it.s.hi, it.s.sink_end, k0, kTileN);
+        const uint32_t full = bar(L::kBarKvFull + slot), to = clear ? bar(L::kBarRaw) : full;
+        pl.copy(is_v ? &tm_v : &tm_k, sRing + slot * L::kTileBytes, to, hk);
+        if (clear) {
+          mbar_wait(to, raw_phase, wc, kErrWaitKV);
           raw_phase ^= 1;
-          const int k0 = it.t.at(j) * kTileN;
           uint8_t* v = gbase + L::kOffRing + slot * L::kTileBytes;
           for (int row = 0; row < kTileN; ++row) {
             if (cache_seen(it.s.lo, it.s.hi, it.s.sink_end, k0 + row, 1)) continue;
@@ -704,17 +707,9 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           __syncwarp();
           if (lane == 0) mbar_arrive(full);
           __syncwarp();
-        } else {
-          copy_tile(it, i, full);
-        }
-        if ((i & 1) && i + 1 < 2 * n_tiles) look_up(it, j + 1);
-      }
-      // give-up path: copies may still be in flight; let them land (bounded) before the shared memory is released
-      if (*abort_flag) {
-        const uint64_t t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 2000000ull) {
         }
       }
+      if (*abort_flag) wait_for_copies();
       __syncwarp();
     }
   }
@@ -728,6 +723,59 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 }
 
 // ---------------------------------------------------------------------------------
+// The rows of a call behind a shared prefix: the pieces that the prefix's launch left and what the launch over the rest of
+// each sequence left, added up and stored.  A warp takes 32 rows of a Q tile and 8 columns of them, a lane a row.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128)
+cache_merge_kernel(const CacheArgs a, int n_parts) {
+  grid_dep_launch();
+  grid_dep_wait();
+  const int r = threadIdx.x, t = blockIdx.x & 1, col = blockIdx.y * 8;
+  const int item = blockIdx.x >> 1, idx = div_by(item, a.by_groups), group = item - idx * a.groups;
+  const int in_tile = div_by(r, a.by_pack), tok = (2 * (a.pairs - 1 - idx) + t) * a.tpt + in_tile;
+  const int head = group * a.pack + (r - in_tile * a.pack);
+  const int rows = a.cu_q != nullptr ? a.total_q : a.B * a.Nq;
+  if (in_tile >= a.tpt || tok >= rows) return;
+  if (a.cu_q != nullptr && (tok < a.cu_q[0] || tok >= a.cu_q[a.B])) return;  // no sequence's
+  auto slot_row = [&](int p) { return ((static_cast<long long>(item) * n_parts + p) * 2 + t) * kTileM + r; };
+  const long long rest = static_cast<long long>(tok) * a.Hq + head;
+  const float2 ml_rest = a.rest_ml[rest];
+  float m = ml_rest.x;
+#pragma unroll 4
+  for (int p = 0; p < n_parts; ++p) m = fmaxf(m, a.part_ml[slot_row(p)].x);
+  float l = 0.f, o[8] = {};
+  auto add = [&](float2 ml, float4 y0, float4 y1) {
+    const float w = part_weight(ml.x, m);
+    l = fmaf(ml.y, w, l);
+    o[0] = fmaf(y0.x, w, o[0]);
+    o[1] = fmaf(y0.y, w, o[1]);
+    o[2] = fmaf(y0.z, w, o[2]);
+    o[3] = fmaf(y0.w, w, o[3]);
+    o[4] = fmaf(y1.x, w, o[4]);
+    o[5] = fmaf(y1.y, w, o[5]);
+    o[6] = fmaf(y1.z, w, o[6]);
+    o[7] = fmaf(y1.w, w, o[7]);
+  };
+  const float4* pr = reinterpret_cast<const float4*>(a.rest_o + rest * D + col);
+  add(ml_rest, pr[0], pr[1]);
+#pragma unroll 4
+  for (int p = 0; p < n_parts; ++p) {
+    const long long at = slot_row(p);
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + (at - r) * D) + (col / 4) * kTileM + r;
+    add(a.part_ml[at], po[0], po[kTileM]);
+  }
+  const float f = l > 0.f ? 1.f / l : l;  // a NaN stays one
+  long long seq = 0, at = tok;
+  if (a.cu_q == nullptr) {
+    seq = div_by(tok, a.by_nq);
+    at = tok - seq * a.Nq;
+  }
+  *reinterpret_cast<uint4*>(a.o + seq * a.os[0] + head * a.os[1] + at * a.os[2] + col) =
+      make_uint4(pack2<BF16>(o[0] * f, o[1] * f), pack2<BF16>(o[2] * f, o[3] * f), pack2<BF16>(o[4] * f, o[5] * f),
+                 pack2<BF16>(o[6] * f, o[7] * f));
+  if (col == 0 && a.lse != nullptr) a.lse[seq * a.ls[0] + head * a.ls[1] + at] = row_lse(m, l);
+}
+
 template <int D, bool BF16, bool PREFIX, bool NARROW = false>
 static cudaError_t launch_t(const CUtensorMap* tm, const CacheArgs& a, int items, int parts, cudaStream_t st) {
   auto kern = fwd_cache_ws_kernel<D, BF16, PREFIX, NARROW>;
@@ -754,6 +802,18 @@ cudaError_t launch_fwd_cache_ws(int D, bool bf16, bool prefix, const CUtensorMap
     return bf16 ? launch_d<128, true>(prefix, tm, a, items, parts, st) : launch_d<128, false>(prefix, tm, a, items, parts, st);
   if (D == 64)
     return bf16 ? launch_d<64, true>(prefix, tm, a, items, parts, st) : launch_d<64, false>(prefix, tm, a, items, parts, st);
+  return cudaErrorInvalidValue;
+}
+
+// After launch_fwd_cache_ws over the prefix (`items` x `parts` pieces) and launch_fwd_cache over the rest.
+cudaError_t launch_cache_merge(int D, bool bf16, const CacheArgs& a, int items, int parts, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(items) * 2, a.D / 8);
+  if (D == 128)
+    return bf16 ? launch_overlapped(cache_merge_kernel<128, true>, grid, 128, 0, st, a, parts)
+                : launch_overlapped(cache_merge_kernel<128, false>, grid, 128, 0, st, a, parts);
+  if (D == 64)
+    return bf16 ? launch_overlapped(cache_merge_kernel<64, true>, grid, 128, 0, st, a, parts)
+                : launch_overlapped(cache_merge_kernel<64, false>, grid, 128, 0, st, a, parts);
   return cudaErrorInvalidValue;
 }
 
