@@ -19,6 +19,7 @@ namespace ma {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 2;  // heads of a lane in flight together
 
 template <bool BF16>
 __device__ __forceinline__ void widen(const uint4& w, float (&x)[8]) {
@@ -44,15 +45,21 @@ __device__ __forceinline__ int sequence_of(const AppendArgs& a, int t) {
 
 }  // namespace
 
-template <bool BF16>
-__global__ void __launch_bounds__(kThreads)
+// kWarps warps take a row together: one where the rows fill the GPU (the three loads of a row's lookups, which wait for one
+// another, are then hidden by the other rows of the SM), eight where they do not.  7 prompts of 7261 tokens in all, 32/8 heads of
+// 128: 36.7 us = 5.0 TB/s, 0.76 of the copy rate (49 with a CTA to a row); 4 x 8192 tokens, 16/4 heads of 64: 39.9 us = 5.1
+// TB/s (89).  Two heads of a lane in flight and three CTAs an SM: 1 and 4 took 37.6 and 40.6 us, 4 and 2 34.5 and 41.7, 3 and 3
+// 39.6 and 44.2.  A step of decode (32 rows) takes 2.5 us, a launch and those three loads.
+template <bool BF16, int kWarps>
+__global__ void __launch_bounds__(kThreads, 3)
 append_kernel(const AppendArgs a) {
+  constexpr int kGroup = 32 * kWarps, kRowsPerCta = kThreads / kGroup;
   grid_dep_launch();
   grid_dep_wait();
   const int units = a.D / 16;  // of a head
-  const int lanes = kThreads / units * units;
-  const int tid = threadIdx.x;
-  const int unit = tid - div_by(tid, a.by_units) * units, lane0 = div_by(tid, a.by_units), step = lanes / units;
+  const int lanes = kGroup / units * units, step = kGroup / units;
+  const int tid = threadIdx.x % kGroup;
+  const int head0 = div_by(tid, a.by_units), unit = tid - head0 * units;
   const bool turns = a.rope != nullptr && unit * 16 < a.rot;
   const int half = a.rot / 2;
   // the unit's two runs of 8 elements
@@ -60,7 +67,9 @@ append_kernel(const AppendArgs a) {
   const int e1 = turns && !a.interleaved ? half + unit * 8 : unit * 16 + 8;
   const int heads = 2 * a.Hkv + (a.q != nullptr ? a.Hq : 0);
 
-  for (int t = blockIdx.x; t < a.rows; t += gridDim.x) {
+  for (long long row = static_cast<long long>(blockIdx.x) * kRowsPerCta + threadIdx.x / kGroup; row < a.rows;
+       row += static_cast<long long>(gridDim.x) * kRowsPerCta) {
+    const int t = static_cast<int>(row);
     int b;
     long long first, n_new;
     if (a.cu_q != nullptr) {
@@ -80,67 +89,84 @@ append_kernel(const AppendArgs a) {
     float cs[8], sn[8];
     const bool turn = turns && s.held;
     if (turn) {
-      const float* row = a.rope + static_cast<long long>(s.pos) * a.rot + unit * 8;
+      const float* angles = a.rope + static_cast<long long>(s.pos) * a.rot + unit * 8;
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
-        *reinterpret_cast<float4*>(cs + i) = *reinterpret_cast<const float4*>(row + i);
-        *reinterpret_cast<float4*>(sn + i) = *reinterpret_cast<const float4*>(row + half + i);
+        *reinterpret_cast<float4*>(cs + i) = *reinterpret_cast<const float4*>(angles + i);
+        *reinterpret_cast<float4*>(sn + i) = *reinterpret_cast<const float4*>(angles + half + i);
       }
     }
     const long long seq = a.cu_q != nullptr ? 0 : b, tok = a.cu_q != nullptr ? t : t - first;
-    for (int h = lane0; h < heads; h += step) {
-      const uint16_t* src;
-      uint16_t* dst;
-      bool rotate = turn;
-      if (h < 2 * a.Hkv) {
-        if (!s.held) continue;
-        const int hk = h < a.Hkv ? h : h - a.Hkv;
+    const uint16_t* k = a.k + seq * a.ks[0] + tok * a.ks[2];
+    const uint16_t* v = a.v + seq * a.vs[0] + tok * a.vs[2];
+    const uint16_t* q = a.q + seq * a.qs[0] + tok * a.qs[2];
+    uint16_t* k_to = a.k_cache + s.page * a.kcs[0] + s.at * a.kcs[2];
+    uint16_t* v_to = a.v_cache + s.page * a.vcs[0] + s.at * a.vcs[2];
+    uint16_t* q_to = a.q_out + seq * a.qos[0] + tok * a.qos[2];
+    // K's heads, V's, Q's in a row; kAhead of them in flight together
+    for (int h0 = s.held ? head0 : 2 * a.Hkv + head0; h0 < heads; h0 += kAhead * step) {
+      uint4 w[kAhead][2];
+      uint16_t* to[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int h = h0 + u * step;
+        if (h >= heads) break;
+        const uint16_t* from;
         if (h < a.Hkv) {
-          src = a.k + seq * a.ks[0] + hk * a.ks[1] + tok * a.ks[2];
-          dst = a.k_cache + s.page * a.kcs[0] + hk * a.kcs[1] + s.at * a.kcs[2];
+          from = k + h * a.ks[1];
+          to[u] = k_to + h * a.kcs[1];
+        } else if (h < 2 * a.Hkv) {
+          from = v + (h - a.Hkv) * a.vs[1];
+          to[u] = v_to + (h - a.Hkv) * a.vcs[1];
         } else {
-          src = a.v + seq * a.vs[0] + hk * a.vs[1] + tok * a.vs[2];
-          dst = a.v_cache + s.page * a.vcs[0] + hk * a.vcs[1] + s.at * a.vcs[2];
-          rotate = false;
+          from = q + (h - 2 * a.Hkv) * a.qs[1];
+          to[u] = q_to + (h - 2 * a.Hkv) * a.qos[1];
         }
-      } else {
-        const int hq = h - 2 * a.Hkv;
-        src = a.q + seq * a.qs[0] + hq * a.qs[1] + tok * a.qs[2];
-        dst = a.q_out + seq * a.qos[0] + hq * a.qos[1] + tok * a.qos[2];
+        w[u][0] = *reinterpret_cast<const uint4*>(from + e0);
+        w[u][1] = *reinterpret_cast<const uint4*>(from + e1);
       }
-      uint4 w0 = *reinterpret_cast<const uint4*>(src + e0), w1 = *reinterpret_cast<const uint4*>(src + e1);
-      if (rotate) {
-        float x[8], y[8], u[8], w[8];
-        widen<BF16>(w0, x);
-        widen<BF16>(w1, y);
-        if (a.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            u[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
-            u[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
-            w[2 * i] = y[2 * i] * cs[4 + i] - y[2 * i + 1] * sn[4 + i];
-            w[2 * i + 1] = y[2 * i + 1] * cs[4 + i] + y[2 * i] * sn[4 + i];
-          }
-        } else {
+      for (int u = 0; u < kAhead; ++u) {
+        const int h = h0 + u * step;
+        if (h >= heads) break;
+        if (turn && (h < a.Hkv || h >= 2 * a.Hkv)) {
+          float x[8], y[8], p[8], r[8];
+          widen<BF16>(w[u][0], x);
+          widen<BF16>(w[u][1], y);
+          if (a.interleaved) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            u[i] = x[i] * cs[i] - y[i] * sn[i];
-            w[i] = y[i] * cs[i] + x[i] * sn[i];
+            for (int i = 0; i < 4; ++i) {
+              p[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
+              p[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+              r[2 * i] = y[2 * i] * cs[4 + i] - y[2 * i + 1] * sn[4 + i];
+              r[2 * i + 1] = y[2 * i + 1] * cs[4 + i] + y[2 * i] * sn[4 + i];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              p[i] = x[i] * cs[i] - y[i] * sn[i];
+              r[i] = y[i] * cs[i] + x[i] * sn[i];
+            }
           }
+          w[u][0] = narrow<BF16>(p);
+          w[u][1] = narrow<BF16>(r);
         }
-        w0 = narrow<BF16>(u);
-        w1 = narrow<BF16>(w);
+        *reinterpret_cast<uint4*>(to[u] + e0) = w[u][0];
+        *reinterpret_cast<uint4*>(to[u] + e1) = w[u][1];
       }
-      *reinterpret_cast<uint4*>(dst + e0) = w0;
-      *reinterpret_cast<uint4*>(dst + e1) = w1;
     }
   }
 }
 
+template <bool BF16>
+static cudaError_t launch_append_t(const AppendArgs& a, int sms, cudaStream_t st) {
+  if (a.rows < sms * 8) return launch_overlapped(append_kernel<BF16, 8>, static_cast<unsigned>(a.rows), kThreads, 0, st, a);
+  const int ctas = (a.rows + 7) / 8;
+  return launch_overlapped(append_kernel<BF16, 1>, static_cast<unsigned>(ctas < sms * 6 ? ctas : sms * 6), kThreads, 0, st, a);
+}
+
 cudaError_t launch_append(bool bf16, const AppendArgs& a, int sms, cudaStream_t st) {
-  const unsigned grid = static_cast<unsigned>(a.rows < sms * 8 ? a.rows : sms * 8);
-  return bf16 ? launch_overlapped(append_kernel<true>, grid, kThreads, 0, st, a)
-              : launch_overlapped(append_kernel<false>, grid, kThreads, 0, st, a);
+  return bf16 ? launch_append_t<true>(a, sms, st) : launch_append_t<false>(a, sms, st);
 }
 
 }  // namespace ma
