@@ -151,11 +151,11 @@ def _load() -> C.CDLL:
         getattr(lib, name).restype = C.c_int
     lib.miniattn_linear.argtypes = [C.c_void_p, C.c_void_p]   # a LinearParams by reference, or its bytes
     lib.miniattn_linear.restype = C.c_int
-    lib.miniattn_fwd_cache.argtypes = [C.POINTER(CacheParams), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.miniattn_fwd_cache.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]   # a CacheParams by reference, or its bytes
     lib.miniattn_fwd_cache.restype = C.c_int
     lib.miniattn_fwd_cache_scratch_bytes.argtypes = [C.POINTER(CacheParams)]
     lib.miniattn_fwd_cache_scratch_bytes.restype = C.c_int64
-    lib.miniattn_paged_append.argtypes = [C.POINTER(AppendParams), C.c_void_p]
+    lib.miniattn_paged_append.argtypes = [C.c_void_p, C.c_void_p]   # an AppendParams by reference, or its bytes
     lib.miniattn_paged_append.restype = C.c_int
     lib.miniattn_merge_partials.argtypes = [C.POINTER(MergeParams), C.c_void_p]
     lib.miniattn_merge_partials.restype = C.c_int

@@ -306,20 +306,20 @@ def flash_attn_fwd(
 
 
 _INT32_MAX = 2 ** 31 - 1
-_window_params: dict = {}   # parameter blocks of recent calls with a window, as _param_cache
+_window_forms: dict = {}   # what follows from the form of a call with a window, once checked: the block behind the pointers
+_pack_cache = struct.Struct("@9P").pack   # the pointers of MiniAttnCacheParams
 
 
 def _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q_pos0, k_pos0, window, sinks):
     """``flash_attn_fwd`` with a sliding window."""
     try:
-        key = (q.data_ptr(), k.data_ptr(), v.data_ptr(), q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype,
-               k.dtype, v.dtype, q.get_device(), k.get_device(), v.get_device(),
-               None if out is None else (out.data_ptr(), out.shape, out.stride(), out.dtype, out.get_device()), causal,
-               softmax_scale, layout, return_lse, kernel, q_pos0, k_pos0, window, sinks)
-        hit = _window_params.get(key)
+        key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.get_device(),
+               k.get_device(), v.get_device(), None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()),
+               causal, softmax_scale, layout, kernel, q_pos0, k_pos0, window, sinks)
+        form = _window_forms.get(key)
     except (AttributeError, TypeError, RuntimeError):
-        key = hit = None
-    if hit is None:
+        key = form = None
+    if form is None:
         if window is None:
             raise RuntimeError("sinks are what stays visible outside a window: window is None")
         if not causal:
@@ -334,29 +334,25 @@ def _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q
         if max(*q.shape, *k.shape) > _INT32_MAX:
             raise RuntimeError("sizes must fit in 31 bits")
         p = _lib.CacheParams()
-        p.q, p.k, p.v, p.o, p.status = f.q, f.k, f.v, f.o if out is not None else None, f.status
         p.q_stride[:], p.k_stride[:], p.v_stride[:], p.o_stride[:] = f.q_stride, f.k_stride, f.v_stride, f.o_stride
         p.lse_stride[:] = (f.Hq * f.Nq, f.Nq)
         p.diag = f.q_pos0 - f.k_pos0
         p.B, p.Hq, p.Hkv, p.D, p.Nq, p.Nk = f.B, f.Hq, f.Hkv, f.D, f.Nq, f.Nk
         p.window, p.sinks = int(window), max(0, min(_INT32_MAX, int(sinks) - f.k_pos0))
         p.dtype, p.softmax_scale = f.dtype, f.softmax_scale
-        hit = (p, _cache_scratch_bytes(p, q.device))
-        if len(_window_params) >= _PARAM_CACHE_MAX:
-            _window_params.clear()
+        form = (bytes(p)[9 * struct.calcsize("P"):], _cache_scratch_bytes(p, q.device), (f.B, f.Hq, f.Nq))
+        if len(_window_forms) >= _PARAM_CACHE_MAX:
+            _window_forms.clear()
         if key is not None:
-            _window_params[key] = hit
-    p, need = hit
-    if out is None or return_lse:
-        p = _lib.CacheParams.from_buffer_copy(p)   # the block that is kept stays as it is
-        if out is None:
-            out = torch.empty_like(q)
-            p.o = out.data_ptr()
-    lse = None
-    if return_lse:
-        lse = torch.empty((p.B, p.Hq, p.Nq), dtype=torch.float32, device=q.device)
-        p.lse = lse.data_ptr()
-    _launch_cache(p, need, q.device)
+            _window_forms[key] = form
+    rest, need, lse_shape = form
+    if out is None:
+        out = torch.empty_like(q)
+    lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device) if return_lse else None
+    device = q.device
+    status = _status_words.get(("cuda", device.index))
+    _launch_cache(_pack_cache(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                              (_status_word(device) if status is None else status).data_ptr(), 0, 0, 0) + rest, need, device)
     return (out, lse) if return_lse else out
 
 
@@ -368,20 +364,20 @@ def _cache_scratch_bytes(p, device: torch.device) -> int:
     return need
 
 
-def _launch_cache(p, need: int, device: torch.device) -> None:
-    """``miniattn_fwd_cache`` on the current stream of `device`, with the scratch of that stream."""
+def _launch_cache(block: bytes, need: int, device: torch.device) -> None:
+    """``miniattn_fwd_cache`` of a packed parameter block on the current stream of `device`, with the scratch of that stream."""
     if _current_device() == device.index:
-        rc = _launch_cache_on(p, need, device, _current_raw_stream(device.index))
+        rc = _launch_cache_on(block, need, device, _current_raw_stream(device.index))
     else:
         with torch.cuda.device(device.index):
-            rc = _launch_cache_on(p, need, device, _current_raw_stream(device.index))
+            rc = _launch_cache_on(block, need, device, _current_raw_stream(device.index))
     if rc != _lib.OK:
         _lib.check(rc, "miniattn_fwd_cache")
 
 
-def _launch_cache_on(p, need: int, device: torch.device, stream: int) -> int:
+def _launch_cache_on(block: bytes, need: int, device: torch.device, stream: int) -> int:
     scratch = _scratch_for(device, stream, need)
-    return _lib.lib.miniattn_fwd_cache(_byref(p), scratch.data_ptr(), scratch.numel(), stream)
+    return _lib.lib.miniattn_fwd_cache(block, scratch.data_ptr(), scratch.numel(), stream)
 
 
 # cudaStream_t of torch's current stream on a device without building a Stream object, and the current device

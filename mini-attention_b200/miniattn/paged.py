@@ -20,19 +20,23 @@ are undefined.
 """
 from __future__ import annotations
 
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from .ops import (_DTYPES, _INT32_MAX, _byref, _current_device, _current_raw_stream, _launch_cache, _cache_scratch_bytes,
-                  _status_word)
+from .ops import (_DTYPES, _INT32_MAX, _cache_scratch_bytes, _current_device, _current_raw_stream, _launch_cache, _status_word,
+                  _status_words)
 
-# Parameter blocks of recent calls by everything that goes into one, as ops._param_cache: a serving loop passes the same cache,
-# table and lengths step after step.
-_attend_cache: dict = {}
-_append_cache: dict = {}
-_CACHE_MAX = 256
+# What follows from the shapes, strides, dtypes and devices of a call, once they have been checked: the part of the parameter
+# block behind the pointers, and the scratch that is needed.  A serving loop passes tensors of the same form step after step.
+_attend_forms: dict = {}
+_append_forms: dict = {}
+_FORMS_MAX = 1024
+_pack_attend = struct.Struct("@9P").pack    # the pointers of MiniAttnCacheParams, in one go
+_pack_append = struct.Struct("@11P").pack   # and of MiniAttnAppendParams
+_ATTEND_POINTERS, _APPEND_POINTERS = 9 * struct.calcsize("P"), 11 * struct.calcsize("P")
 
 
 def rope_table(positions: int, dim: int, *, theta: float = 10000.0, device: Union[torch.device, str, None] = None) -> torch.Tensor:
@@ -114,16 +118,17 @@ def _page_strides(t: torch.Tensor) -> Tuple[int, int, int]:
     return t.stride(0), t.stride(2), t.stride(1)
 
 
-def _sig(t: Optional[torch.Tensor]):
-    """What a parameter block holds of a tensor, and what its checks look at."""
-    return None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype, t.get_device())
+def _form(t: Optional[torch.Tensor]):
+    """What the checks look at."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
-def _launch(device_index: int, call):
-    if _current_device() == device_index:
-        return call(_current_raw_stream(device_index))
-    with torch.cuda.device(device_index):
-        return call(_current_raw_stream(device_index))
+def _keep(forms: dict, key, value):
+    if key is not None:
+        if len(forms) >= _FORMS_MAX:
+            forms.clear()
+        forms[key] = value
+    return value
 
 
 def paged_append(
@@ -152,12 +157,12 @@ def paged_append(
     Returns the rotated queries, or None without ``q``.
     """
     try:
-        key = (_sig(k), _sig(v), _sig(k_cache), _sig(v_cache), _sig(block_table), _sig(seq_lens), _sig(cu_q), _sig(q),
-               _sig(q_out), _sig(rope), interleaved)
-        p = _append_cache.get(key)
+        key = (_form(k), _form(v), _form(k_cache), _form(v_cache), _form(block_table), _form(seq_lens), _form(cu_q), _form(q),
+               _form(q_out), _form(rope), interleaved)
+        form = _append_forms.get(key)
     except (AttributeError, TypeError, RuntimeError):   # not tensors: let the checks below say so
-        key = p = None
-    if p is None:
+        key = form = None
+    if form is None:
         _check_half("k", k, None, 4 if cu_q is None else 3)
         _check_half("v", v, k, k.dim())
         B = _check_paged(k, k_cache, v_cache, block_table, seq_lens, cu_q)
@@ -180,13 +185,6 @@ def paged_append(
             if rope.dtype != torch.float32 or not rope.is_contiguous():
                 raise RuntimeError("rope must be a contiguous fp32 table")
         p = _lib.AppendParams()
-        p.k, p.v, p.k_cache, p.v_cache = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-        p.q = q.data_ptr() if q is not None else None
-        p.q_out = q_out.data_ptr() if q_out is not None else None
-        p.rope = rope.data_ptr() if rope is not None else None
-        p.status = _status_word(k.device).data_ptr()
-        p.block_table, p.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
-        p.cu_q = cu_q.data_ptr() if cu_q is not None else None
         p.k_stride[:], p.v_stride[:] = _token_strides(k), _token_strides(v)
         if q is not None:
             p.q_stride[:] = _token_strides(q)
@@ -200,16 +198,22 @@ def paged_append(
         p.interleaved = 1 if interleaved else 0
         p.page_size, p.n_pages, p.table_width = k_cache.shape[1], k_cache.shape[0], block_table.shape[1]
         p.dtype = _DTYPES[k.dtype]
-        if key is not None and k.numel() > 0:
-            if len(_append_cache) >= _CACHE_MAX:
-                _append_cache.clear()
-            _append_cache[key] = p
+        form = _keep(_append_forms, key, bytes(p)[_APPEND_POINTERS:])
     if q is not None and q_out is None:
         q_out = torch.empty_like(q)
-        p = _lib.AppendParams.from_buffer_copy(p)   # the block that is kept stays as it is
-        p.q_out = q_out.data_ptr()
     if k.numel() > 0:
-        rc = _launch(k.get_device(), lambda stream: _lib.lib.miniattn_paged_append(_byref(p), stream))
+        device = k.device
+        status = _status_words.get(("cuda", device.index))
+        block = _pack_append(
+            k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            0 if q is None else q_out.data_ptr(), 0 if rope is None else rope.data_ptr(),
+            (_status_word(device) if status is None else status).data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            0 if cu_q is None else cu_q.data_ptr()) + form
+        if _current_device() == device.index:
+            rc = _lib.lib.miniattn_paged_append(block, _current_raw_stream(device.index))
+        else:
+            with torch.cuda.device(device):
+                rc = _lib.lib.miniattn_paged_append(block, _current_raw_stream(device.index))
         if rc != _lib.OK:
             _lib.check(rc, "miniattn_paged_append")
     return q_out
@@ -246,12 +250,12 @@ def paged_attention(
     with ``cu_q``.  A NaN or infinity among the values of a key that any row of a sequence sees may show in others of its rows.
     """
     try:
-        key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(block_table), _sig(seq_lens), _sig(cu_q), _sig(out), max_q, window,
-               sinks, shared_len, softmax_scale, return_lse)
-        hit = _attend_cache.get(key)
+        key = (_form(q), _form(k_cache), _form(v_cache), _form(block_table), _form(seq_lens), _form(cu_q), _form(out), max_q,
+               window, sinks, shared_len, softmax_scale)
+        form = _attend_forms.get(key)
     except (AttributeError, TypeError, RuntimeError):
-        key = hit = None
-    if hit is None:
+        key = form = None
+    if form is None:
         _check_half("q", q, None, 4 if cu_q is None else 3)
         B = _check_paged(q, k_cache, v_cache, block_table, seq_lens, cu_q)
         Hq, Hkv = q.shape[-2], k_cache.shape[2]
@@ -262,11 +266,8 @@ def paged_attention(
             if out.shape != q.shape:
                 raise RuntimeError("out must match q in shape")
         p = _lib.CacheParams()
-        p.q, p.k, p.v = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-        p.o = out.data_ptr() if out is not None else None
-        p.status = _status_word(q.device).data_ptr()
-        p.block_table, p.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
-        p.cu_q = cu_q.data_ptr() if cu_q is not None else None
+        # compared with null by the question for the scratch; what is launched gets its pointers below
+        p.block_table, p.seq_lens, p.cu_q = block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr()
         p.q_stride[:] = _token_strides(q)
         p.o_stride[:] = _token_strides(out if out is not None else torch.empty_like(q))
         p.k_stride[:], p.v_stride[:] = _page_strides(k_cache), _page_strides(v_cache)
@@ -284,21 +285,18 @@ def paged_attention(
         p.sinks, p.shared_len = _whole("sinks", sinks, 0), _whole("shared_len", shared_len, 0)
         p.dtype = _DTYPES[q.dtype]
         p.softmax_scale = float(softmax_scale) if softmax_scale is not None else 0.0
-        hit = (p, _cache_scratch_bytes(p, q.device))
-        if key is not None:
-            if len(_attend_cache) >= _CACHE_MAX:
-                _attend_cache.clear()
-            _attend_cache[key] = hit
-    p, need = hit
-    if out is None or return_lse:
-        p = _lib.CacheParams.from_buffer_copy(p)
-        if out is None:
-            out = torch.empty_like(q)
-            p.o = out.data_ptr()
-    lse = None
-    if return_lse:
-        lse = torch.empty((p.B, p.Hq, p.Nq) if cu_q is None else (p.Hq, p.total_q), dtype=torch.float32, device=q.device)
-        p.lse = lse.data_ptr()
+        need = _cache_scratch_bytes(p, q.device)
+        lse_shape = (B, Hq, q.shape[1]) if cu_q is None else (Hq, q.shape[0])
+        form = _keep(_attend_forms, key, (bytes(p)[_ATTEND_POINTERS:], need, lse_shape))
+    rest, need, lse_shape = form
+    if out is None:
+        out = torch.empty_like(q)
+    lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device) if return_lse else None
     if q.numel() > 0:
-        _launch_cache(p, need, q.device)
+        device = q.device
+        status = _status_words.get(("cuda", device.index))
+        _launch_cache(_pack_attend(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            (_status_word(device) if status is None else status).data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            0 if cu_q is None else cu_q.data_ptr()) + rest, need, device)
     return (out, lse) if return_lse else out
