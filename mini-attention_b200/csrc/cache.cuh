@@ -119,7 +119,7 @@ __host__ __device__ inline CacheTiles cache_tiles(int lo, int hi, int sink_end) 
 
 // Whether [k, k + n) holds keys that no row sees.
 __host__ __device__ inline bool cache_partly_seen(int lo, int hi, int sink_end, int k, int n) {
-  return k + n > hi || (k < lo && k + n > sink_end);
+  return k + n > hi || (k < lo && sink_end < lo && k + n > sink_end);
 }
 
 // Whether some row sees one of the keys [k, k + n).

@@ -12,6 +12,9 @@ ones that share their input run as one launch.
 * ``GQA_Flash``  kernels/standard/pytorch/gqa.py:7-51   (causal; K/V heads are broadcast inside
                  the kernel instead of ``repeat_interleave``)
 * ``MQA_Flash``  kernels/standard/pytorch/mqa.py:8-47   (causal; single K/V head)
+
+``forward_paged`` of the last two serves new tokens of many sequences against a paged cache (no counterpart in the
+reference): projections, rotation and append, attention over the pages, output projection.
 """
 from __future__ import annotations
 
@@ -21,6 +24,7 @@ import torch.nn as nn
 import math
 
 from .ops import flash_attn_fwd, linear
+from .paged import paged_append, paged_attention
 
 
 def _attend(q, k, v, causal, return_lse=False):
@@ -32,6 +36,21 @@ def _attend(q, k, v, causal, return_lse=False):
     o = res[0] if return_lse else res
     o = o.reshape(o.shape[0], o.shape[1], -1)
     return (o, res[1]) if return_lse else o
+
+
+def _serve(projected, w_o, n_kv_heads, head_dim, k_cache, v_cache, block_table, seq_lens, cu_q, max_q, rope, interleaved, window,
+           sinks, shared_len):
+    """The rest of ``forward_paged`` after the projections of q and of k and v."""
+    q, kv = projected
+    rows = q.shape[:-1]
+    q = q.view(*rows, -1, head_dim)
+    kv = kv.view(*rows, 2, n_kv_heads, head_dim)
+    turned = q if rope is not None else None   # in place: nobody else has seen it
+    paged_append(kv[..., 0, :, :], kv[..., 1, :, :], k_cache, v_cache, block_table, seq_lens, cu_q=cu_q, q=turned, q_out=turned,
+                 rope=rope, interleaved=interleaved)
+    o = paged_attention(q, k_cache, v_cache, block_table, seq_lens, cu_q=cu_q, max_q=max_q, window=window, sinks=sinks,
+                        shared_len=shared_len)
+    return _project(o.reshape(*rows, -1), w_o, projected)
 
 
 def _project(o, layer, projected):
@@ -101,6 +120,15 @@ class GQA_Flash(nn.Module):
         kv = kv.view(B, S, 2, self.n_kv_heads, self.head_dim)
         return _project(_attend(q, kv[:, :, 0], kv[:, :, 1], True), self.w_o, projected)
 
+    def forward_paged(self, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                      seq_lens: torch.Tensor, *, cu_q=None, max_q=None, rope=None, interleaved: bool = False, window=None,
+                      sinks: int = 0, shared_len: int = 0) -> torch.Tensor:
+        """New tokens x, (B, n, d_model) or (rows, d_model) with ``cu_q``, of sequences whose keys and values lie in pages: theirs
+        are appended (``seq_lens`` counts them already) and they attend to everything their sequences hold, as
+        :func:`miniattn.paged_append` and :func:`miniattn.paged_attention` say."""
+        return _serve(linear(x, self.w_q, self.kv), self.w_o, self.n_kv_heads, self.head_dim, k_cache, v_cache, block_table, seq_lens, cu_q,
+                      max_q, rope, interleaved, window, sinks, shared_len)
+
 
 class MQA_Flash(nn.Module):
     def __init__(self, d_model: int, n_heads: int):
@@ -117,3 +145,12 @@ class MQA_Flash(nn.Module):
         q = q.view(B, S, self.n_heads, self.head_dim)
         kv = kv.view(B, S, 2, 1, self.head_dim)
         return _project(_attend(q, kv[:, :, 0], kv[:, :, 1], True), self.w_o, projected)
+
+    def forward_paged(self, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                      seq_lens: torch.Tensor, *, cu_q=None, max_q=None, rope=None, interleaved: bool = False, window=None,
+                      sinks: int = 0, shared_len: int = 0) -> torch.Tensor:
+        """New tokens x, (B, n, d_model) or (rows, d_model) with ``cu_q``, of sequences whose keys and values lie in pages: theirs
+        are appended (``seq_lens`` counts them already) and they attend to everything their sequences hold, as
+        :func:`miniattn.paged_append` and :func:`miniattn.paged_attention` say."""
+        return _serve(linear(x, self.w_q, self.k_v), self.w_o, 1, self.head_dim, k_cache, v_cache, block_table, seq_lens, cu_q,
+                      max_q, rope, interleaved, window, sinks, shared_len)
