@@ -33,6 +33,7 @@ constexpr int kBox = kKeys * 128;    // one [64 keys x 128 B] box
 constexpr float kLazy = 8.0f;        // log2 units a row's maximum may move before O is rescaled
 constexpr int kMergePitch = 36;      // floats per row of the merge buffer (32 + padding)
 constexpr int kPiece = 8;            // tiles of a piece where every CTA works on one
+constexpr int kItemCost = 3;         // what an item takes beside its tiles, in tiles
 
 template <int D>
 struct Layout {
@@ -43,7 +44,8 @@ struct Layout {
   static constexpr int kOffMl = kOffMerge + 4 * 16 * kMergePitch * 4;  // float2[4 warps][16]
   static constexpr int kOffBar = kOffMl + 4 * 16 * 8;                  // full[kStages], empty[kStages]
   static constexpr int kOffScan = kOffBar + 2 * kStages * 8;           // long long[2][4 warps], tiles before the first sequence
-  static constexpr int kOffMisc = kOffScan + 10 * 8;                   // abort flag, arrival order, first sequence
+  static constexpr int kOffWalk = kOffScan + 10 * 8;                   // Walk of the first sequence
+  static constexpr int kOffMisc = kOffWalk + 80;                       // abort flag, arrival order, first sequence
   static constexpr int kBytes = kOffMisc + 16;
   static constexpr int kDynSmem = kBytes + 1024;
 };
@@ -76,8 +78,9 @@ __device__ __forceinline__ float row_lse(float m, float l) {
   return l == 0.f ? -INFINITY : m * 0.6931471805599453f + __logf(l);
 }
 
-// Sequence b of the call, and how its items are counted: n_rb row blocks per KV head, `slots` places of the launch's tiles
-// for each (its t.n tiles and, where a launch is so short that a CTA works on one piece, what fills the last piece up).
+// Sequence b of the call, and how its items are counted: n_rb row blocks per KV head, `slots` places on the launch's line for
+// each: its t.n tiles and kItemCost more for its start and end, or, where a launch is so short that every CTA works on one
+// piece, what fills the last piece up.
 struct Walk {
   CacheSeq s;
   CacheTiles t;
@@ -86,6 +89,7 @@ struct Walk {
     return static_cast<long long>(a.Hkv) * n_rb * slots;
   }
 };
+static_assert(sizeof(Walk) <= 80, "Walk");
 template <int kRows>
 __device__ __forceinline__ Walk walk_to(const CacheArgs& a, int b, bool pieces) {
   Walk w;
@@ -97,7 +101,7 @@ __device__ __forceinline__ Walk walk_to(const CacheArgs& a, int b, bool pieces) 
   w.s = cache_seq(a, r0, r1, a.seq_lens != nullptr ? a.seq_lens[b] : 0);
   w.t = cache_tiles<kKeys>(w.s.lo, w.s.hi, w.s.sink_end);
   w.n_rb = static_cast<int>((static_cast<long long>(w.s.nq) * a.G + kRows - 1) / kRows);
-  w.slots = pieces ? (w.t.n + (kPiece - 1)) / kPiece * kPiece : w.t.n;
+  w.slots = pieces ? (w.t.n + (kPiece - 1)) / kPiece * kPiece : w.t.n + kItemCost;
   return w;
 }
 
@@ -145,12 +149,14 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const int b0 = min(a.B, tid * run), b1 = tid < 128 ? min(a.B, b0 + run) : b0;
   long long mine = 0, mine_pieces = 0;
   bool bad = false;
+  Walk own{};
   for (int b = b0; b < b1; ++b) {
     const Walk w = walk_to<kRows>(a, b, true);
     const long long items = static_cast<long long>(a.Hkv) * w.n_rb;
-    mine += items * w.t.n;
+    mine += items * (w.t.n + kItemCost);
     mine_pieces += items * w.slots;
     bad |= w.s.bad;
+    if (run == 1) own = w;
   }
   if (bad && a.status != nullptr) atomicOr(a.status, kErrCache);
   long long before = mine, before_pieces = mine_pieces;  // inclusive over the warp, then exclusive over the CTA
@@ -190,23 +196,29 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (lo >= hi) return;
   if (tid < 128 && lo >= before && lo < before + mine) {
     int b = b0;
-    for (;; ++b) {
-      const long long n = walk_to<kRows>(a, b, pieces).total(a);
-      if (lo < before + n) break;
-      before += n;
+    if (run == 1) {
+      if (!pieces) own.slots = own.t.n + kItemCost;
+    } else {
+      for (;; ++b) {
+        own = walk_to<kRows>(a, b, pieces);
+        const long long n = own.total(a);
+        if (lo < before + n || b + 1 >= b1) break;
+        before += n;
+      }
     }
     *first_seq = b;
     scan[8] = before;
+    *reinterpret_cast<Walk*>(gbase + L::kOffWalk) = own;
   }
   __syncthreads();
   int b = *first_seq;
-  long long base = scan[8];  // tiles before sequence b
-  Walk w = walk_to<kRows>(a, b, pieces);
-  auto next_seq = [&]() {  // the next sequence that has rows; only while tiles are left
+  long long base = scan[8];  // places before sequence b
+  Walk w = *reinterpret_cast<const Walk*>(gbase + L::kOffWalk);
+  auto next_seq = [&]() {  // the next sequence that has rows; only while places are left
     do {
       base += w.total(a);
       w = walk_to<kRows>(a, ++b, pieces);
-    } while (w.n_rb == 0);
+    } while (w.n_rb == 0 && b + 1 < a.B);
   };
 
   if (warp == 4) {
@@ -238,11 +250,24 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
       }
     };
-    look_up();
-    int slot = 0, par = 1, i = 0;
-    // with pieces, hi may lie past the item's last tile: the CTA has none after it
-    const int n_mine = static_cast<int>(pieces ? min(hi - lo, static_cast<long long>(w.t.n - j)) : hi - lo);
-    for (; i < n_mine; ++i) {
+    long long x = lo;
+    auto to_a_tile = [&]() {  // past the places of items that hold no tile
+      while (x < hi && j >= w.t.n) {
+        x += w.slots - j;
+        j = 0;
+        if (x < hi && ++rb == w.n_rb) {
+          rb = 0;
+          if (++hk == a.Hkv) {
+            hk = 0;
+            next_seq();
+          }
+        }
+      }
+    };
+    to_a_tile();
+    if (x < hi) look_up();
+    int slot = 0, par = 1;
+    for (int i = 0; x < hi; ++i) {
       if (i >= L::kStages) mbar_wait(empty(slot), par, wc, kErrWaitFree);
       const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, wanted));
       if (lane == 0) mbar_expect_tx(full(slot), n_copies * box_bytes);
@@ -253,19 +278,10 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         slot = 0;
         par ^= 1;
       }
-      if (i + 1 < n_mine) {
-        if (++j == w.t.n) {
-          j = 0;
-          if (++rb == w.n_rb) {
-            rb = 0;
-            if (++hk == a.Hkv) {
-              hk = 0;
-              next_seq();
-            }
-          }
-        }
-        look_up();
-      }
+      ++x;
+      ++j;
+      to_a_tile();
+      if (x < hi) look_up();
     }
     // give-up path: let the copies in flight land (bounded) before the shared memory is released
     if (*abort_flag) {
@@ -294,6 +310,10 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const long long item0 = base + it * w.slots;
     const int t0 = static_cast<int>(x - item0);
     const int t1 = static_cast<int>(min(static_cast<long long>(w.t.n), hi - item0));
+    if (t0 >= w.t.n) {  // places that hold no tile
+      x = item0 + w.slots;
+      continue;
+    }
     const int hk = static_cast<int>(cache_div(it, w.n_rb)), rb = static_cast<int>(it - static_cast<long long>(hk) * w.n_rb);
     const int rows = w.s.nq * a.G, row0 = rb * kRows;
 
@@ -510,42 +530,68 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       y.y = pack2<BF16>(o.z, o.w);
       *reinterpret_cast<uint2*>(a.o + b * a.os[0] + h * a.os[1] + (w.s.row0 + tok) * a.os[2] + col) = y;
     };
+    if (RG == 1 && rows - row0 <= 4) {
+      // the four key groups of at most four rows fit the buffer at once: [warp][4 rows][D]
+      if (g < 4) {
 #pragma unroll
-    for (int p = 0; p < D / 32; ++p) {  // 32 columns at a time through 9 KB
-      float* mine_s = merge + warp * 16 * kMergePitch;
-#pragma unroll
-      for (int jj = 0; jj < 4; ++jj) {
-        const int n = p * 4 + jj;
-        *reinterpret_cast<float2*>(mine_s + g * kMergePitch + jj * 8 + tig * 2) =
-            make_float2(acc[n][0] * f[0], acc[n][1] * f[0]);
-        *reinterpret_cast<float2*>(mine_s + (g + 8) * kMergePitch + jj * 8 + tig * 2) =
-            make_float2(acc[n][2] * f[1], acc[n][3] * f[1]);
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(merge + (warp * 4 + g) * (D + 4) + n * 8 + tig * 2) =
+              make_float2(acc[n][0] * f[0], acc[n][1] * f[0]);
       }
       workers_sync();
-      const int rr = tid >> 3, c4 = (tid & 7) * 4;
-#pragma unroll
-      for (int rgi = 0; rgi < RG; ++rgi) {
-        const int r_in = rgi * 16 + rr;
-        if (row0 + r_in >= rows) continue;
+      const int r_in = tid / (D / 4), col = (tid % (D / 4)) * 4;
+      for (int rr = r_in; rr < rows - row0; rr += 512 / D) {
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < KG; ++k) {
-          const float4 y = *reinterpret_cast<const float4*>(merge + ((k * RG + rgi) * 16 + rr) * kMergePitch + c4);
+          const float4 y = *reinterpret_cast<const float4*>(merge + (k * 4 + rr) * (D + 4) + col);
           o.x += y.x;
           o.y += y.y;
           o.z += y.z;
           o.w += y.w;
         }
-        const int col = p * 32 + c4;
-        if (!whole) *reinterpret_cast<float4*>(a.part_o + (my_slot * kRows + r_in) * D + col) = o;
-        else store_row(r_in, col, o);
+        if (!whole) *reinterpret_cast<float4*>(a.part_o + (my_slot * kRows + rr) * D + col) = o;
+        else store_row(rr, col, o);
       }
       workers_sync();
+    } else {
+#pragma unroll
+      for (int p = 0; p < D / 32; ++p) {  // 32 columns at a time through 9 KB
+        float* mine_s = merge + warp * 16 * kMergePitch;
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          const int n = p * 4 + jj;
+          *reinterpret_cast<float2*>(mine_s + g * kMergePitch + jj * 8 + tig * 2) =
+              make_float2(acc[n][0] * f[0], acc[n][1] * f[0]);
+          *reinterpret_cast<float2*>(mine_s + (g + 8) * kMergePitch + jj * 8 + tig * 2) =
+              make_float2(acc[n][2] * f[1], acc[n][3] * f[1]);
+        }
+        workers_sync();
+        const int rr = tid >> 3, c4 = (tid & 7) * 4;
+#pragma unroll
+        for (int rgi = 0; rgi < RG; ++rgi) {
+          const int r_in = rgi * 16 + rr;
+          if (row0 + r_in >= rows) continue;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < KG; ++k) {
+            const float4 y = *reinterpret_cast<const float4*>(merge + ((k * RG + rgi) * 16 + rr) * kMergePitch + c4);
+            o.x += y.x;
+            o.y += y.y;
+            o.z += y.z;
+            o.w += y.w;
+          }
+          const int col = p * 32 + c4;
+          if (!whole) *reinterpret_cast<float4*>(a.part_o + (my_slot * kRows + r_in) * D + col) = o;
+          else store_row(r_in, col, o);
+        }
+        workers_sync();
+      }
     }
     if (!whole) {
       __threadfence();  // release: the piece before the count
       workers_sync();
-      const int n_parts = static_cast<int>(cache_div(item0 + w.slots - 1, share) - c_first + 1);
+      const int n_parts = static_cast<int>(cache_div(item0 + w.t.n - 1, share) - c_first + 1);
       if (tid == 0) {
         __threadfence();
         *order = atomicAdd(a.counters + c_first, 1);

@@ -741,7 +741,7 @@ cache_merge_kernel(const CacheArgs a, int n_parts) {
   const long long rest = static_cast<long long>(tok) * a.Hq + head;
   const float2 ml_rest = a.rest_ml[rest];
   float m = ml_rest.x;
-#pragma unroll 4
+#pragma unroll 8
   for (int p = 0; p < n_parts; ++p) m = fmaxf(m, a.part_ml[slot_row(p)].x);
   float l = 0.f, o[8] = {};
   auto add = [&](float2 ml, float4 y0, float4 y1) {
@@ -758,11 +758,21 @@ cache_merge_kernel(const CacheArgs a, int n_parts) {
   };
   const float4* pr = reinterpret_cast<const float4*>(a.rest_o + rest * D + col);
   add(ml_rest, pr[0], pr[1]);
-#pragma unroll 4
-  for (int p = 0; p < n_parts; ++p) {
-    const long long at = slot_row(p);
-    const float4* po = reinterpret_cast<const float4*>(a.part_o + (at - r) * D) + (col / 4) * kTileM + r;
-    add(a.part_ml[at], po[0], po[kTileM]);
+  constexpr int kAhead = 6;  // pieces whose loads are in flight together
+  for (int p0 = 0; p0 < n_parts; p0 += kAhead) {
+    float4 y[kAhead][2];
+    float2 ml[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const long long at = slot_row(min(p0 + u, n_parts - 1));
+      const float4* po = reinterpret_cast<const float4*>(a.part_o + (at - r) * D) + (col / 4) * kTileM + r;
+      ml[u] = a.part_ml[at];
+      y[u][0] = po[0];
+      y[u][1] = po[kTileM];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (p0 + u < n_parts) add(ml[u], y[u][0], y[u][1]);
   }
   const float f = l > 0.f ? 1.f / l : l;  // a NaN stays one
   long long seq = 0, at = tok;
