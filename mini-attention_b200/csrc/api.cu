@@ -1030,9 +1030,9 @@ static int check_cache_sizes(const MiniAttnCacheParams* p) {
 namespace {
 // Which kernels a call over a cache runs.  Decided by sizes alone: lengths are known on the device only.
 struct CachePlan {
-  // rows of all sequences: fwd_cache.cu with rg groups of 16 rows, or (rg = 0) fwd_cache_ws.cu in `items` x `parts` CTAs
+  // rows of all sequences: fwd_cache.cu with rg groups of 16 rows, or (rg = 0) fwd_cache_ws.cu in ctas x parts CTAs
   int rg, n_ctas;
-  int items, parts, pairs;
+  int ctas, parts, pairs, pair_items, cut;
   // a launch over the shared prefix before it and one after it that adds its pieces (pre_items = 0: none)
   int pre_items, pre_parts, pre_pairs;
   int pack, tpt, groups;
@@ -1049,7 +1049,7 @@ constexpr int kMinPieceTiles = 4;      // 128-key tiles of a piece
 constexpr int kMinPrefixTiles = 2;     // of a shared prefix's, whose pieces a launch of its own adds up
 constexpr long long kMaxPieces = 480;  // of all items together: 64 MB of scratch at D = 128
 
-// Pieces that items of at most `tiles` tiles are cut into.  A CTA takes its tiles and about 4 steps of a tile's time beside
+// Pieces that items of at most `tiles` tiles are cut into where all are alike.  A CTA takes its tiles and about 4 steps of a tile's time beside
 // them; a piece takes 2 more to leave its result, the last 0.8 for each piece it folds.
 int cache_pieces(long long items, int tiles, int sms) {
   int best = 1;
@@ -1094,11 +1094,26 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
   }
   c.pairs = static_cast<int>((n + span - 1) / span);
   const long long items = (ragged ? p->total_q / span + p->B : static_cast<long long>(p->B) * c.pairs) * c.groups;
-  const long long likely = ragged ? (p->total_q / span + (p->B + 1) / 2) * c.groups : items;
-  c.items = static_cast<int>(std::min<long long>(items, 0x7fffffff));
+  c.ctas = c.pair_items = static_cast<int>(std::min<long long>(items, 0x7fffffff));
+  c.parts = 1;
+  if (ragged) {
+    if (items <= kMaxPieces) {  // many more come out even without
+      c.cut = 2 * sms;
+      c.ctas += c.cut;
+      c.part_rows = static_cast<size_t>(c.ctas) * 2 * ma::kTileM;
+    }
+    return c;
+  }
   const long long seen = p->window > 0 ? std::min(room, static_cast<long long>(p->window) + p->sinks + span + 256) : room;
-  c.parts = items <= 2000 ? cache_pieces(std::max<long long>(likely, 1), tiles_of(seen), sms) : 1;
+  if (items <= kMaxPieces) c.parts = cache_pieces(items, tiles_of(seen), sms);
   if (c.parts > 1) c.part_rows = static_cast<size_t>(items) * c.parts * 2 * ma::kTileM;
+  // A last wave that is at most half full: its pairs are taken apart, so that it ends sooner (not where a sequence has an odd
+  // number of Q tiles: half of the CTAs would have nothing to do).
+  const long long rest = items % sms;
+  if (c.parts == 1 && items > sms && rest > 0 && 2 * rest <= sms && (n + c.tpt - 1) / c.tpt % 2 == 0 && items < 0x3fffffff) {
+    c.pair_items = static_cast<int>(items - rest);
+    c.ctas = static_cast<int>(items + rest);
+  }
   return c;
 }
 }  // namespace
@@ -1211,13 +1226,14 @@ int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scrat
   };
   CUtensorMap tm[4] = {};
   cudaError_t e = cudaSuccess;
-  const auto pairs_of = [&](int pairs) {
+  const auto pairs_of = [&](int pairs, int pair_items) {
     a.pairs = pairs;
     a.by_pairs = ma::fast_div(pairs > 0 ? pairs : 1);
+    a.pair_items = pair_items;
   };
   if (plan.pre_items > 0) {
     if ((rc = cache_ws_maps(p, plan, dt, true, tm)) != 0 || (rc = kv_maps(tm + 1, 128)) != 0) return rc;
-    pairs_of(plan.pre_pairs);
+    pairs_of(plan.pre_pairs, plan.pre_items);
     a.part_ml = pre_ml;
     a.part_o = pre_o;
     a.min_tiles = 1;
@@ -1234,8 +1250,9 @@ int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scrat
     e = ma::launch_fwd_cache(Dk, bf16, tm, a, plan.rg, plan.n_ctas, st);
   } else {
     if ((rc = cache_ws_maps(p, plan, dt, p->cu_q != nullptr, tm)) != 0 || (rc = kv_maps(tm + 1, 128)) != 0) return rc;
-    pairs_of(plan.pairs);
-    e = ma::launch_fwd_cache_ws(Dk, bf16, false, tm, a, plan.items, plan.parts, st);
+    pairs_of(plan.pairs, plan.pair_items);
+    a.cut = plan.cut;
+    e = ma::launch_fwd_cache_ws(Dk, bf16, false, tm, a, plan.ctas, plan.parts, st);
   }
   if (e == cudaSuccess && plan.pre_items > 0) {
     a.part_ml = pre_ml;

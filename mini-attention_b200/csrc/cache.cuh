@@ -30,6 +30,8 @@ struct CacheArgs {
   // fwd_cache_ws.cu: query heads that share a Q tile (all G of a KV head, or 1), tokens of each in it, pairs of Q tiles of a
   // sequence (not ragged), groups of `pack` heads, tiles that a piece of an item has at least
   int pack, tpt, pairs, groups, min_tiles;
+  int pair_items;          // not ragged: CTAs before this one take two Q tiles, those from it on one each
+  int cut;                 // ragged: items are cut so that all together make about this many pieces (0: not)
   FastDiv by_pack, by_pairs, by_groups, by_gqa;
   int shared;              // a launch over a shared prefix: its tokens
   // scratch: pieces of cut items, un-normalised

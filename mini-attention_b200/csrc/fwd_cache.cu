@@ -32,7 +32,7 @@ constexpr int kKeys = 64;            // keys per tile
 constexpr int kBox = kKeys * 128;    // one [64 keys x 128 B] box
 constexpr float kLazy = 8.0f;        // log2 units a row's maximum may move before O is rescaled
 constexpr int kMergePitch = 36;      // floats per row of the merge buffer (32 + padding)
-constexpr int kPiece = 8;            // tiles of a piece where every CTA works on one
+constexpr int kPiece = 4;            // tiles of a piece where every CTA works on one
 constexpr int kItemCost = 3;         // what an item takes beside its tiles, in tiles
 
 template <int D>

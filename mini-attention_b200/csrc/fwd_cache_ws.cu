@@ -64,7 +64,7 @@ struct WsItem {
   CacheTiles t;
   int b, q0, nt, group;     // sequence, first query token, Q tiles that hold rows (0: no item), group of heads
   int j0, n;                // tiles [j0, j0 + n) of t
-  int part, n_parts, item;  // piece of the item, pieces in all, number of the item
+  int part, n_parts, slot0; // piece of the item, pieces in all, slot of scratch of the first
 };
 static_assert(sizeof(WsItem) <= 96, "WsItem");
 
@@ -133,36 +133,62 @@ __device__ __forceinline__ void wait_for_copies() {
   }
 }
 
-// Sequence and pair of Q tiles of pair number `idx` of a ragged launch; the whole warp.  False: fewer pairs than that.
-__device__ __forceinline__ bool ragged_pair(const CacheArgs& a, int idx, int* b, int* pair, CacheSeq* s) {
+// Which piece of which item CTA x of a ragged launch works on; the whole warp.  False: none.  Lengths are known here only, so
+// every CTA adds up the tiles of all sequences: pieces are at most half as long as an SM's share, and where the sequences are
+// few those with the most keys come first.  (One piece per pair, sequences in their order: 148 SMs wait for the last of 192
+// items of 100 tiles, 357 us where all items together are 237 on each SM.)
+__device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* it, int* pair) {
   const int lane = threadIdx.x & 31, span = 2 * a.tpt;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int bb = b0 + lane;
-    int r0 = 0, r1 = 0, n = 0;
-    if (bb < a.B) {
-      r0 = a.cu_q[bb];
-      r1 = a.cu_q[bb + 1];
-      const int c0 = clamp_to(r0, 0, a.total_q), c1 = clamp_to(r1, c0, a.total_q);
-      n = (c1 - c0 + (span - 1)) / span;
+  auto look = [&](int b, CacheSeq* s, int* pairs, int* tiles) {
+    *pairs = 0;
+    *tiles = 1;
+    if (b >= a.B) return;
+    *s = cache_seq(a, a.cu_q[b], a.cu_q[b + 1], a.seq_lens[b]);
+    *pairs = (s->nq + (span - 1)) / span;
+    long long seen = s->hi;
+    if (a.window > 0) seen = min(seen, static_cast<long long>(a.window) + span + a.sinks + kTileN);
+    *tiles = max(1, static_cast<int>((seen + (kTileN - 1)) / kTileN));
+  };
+  CacheSeq s{};
+  int pairs, tiles, most = 0x7fffffff;  // tiles of a piece
+  if (a.cut > 0) {
+    long long total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      look(b0 + lane, &s, &pairs, &tiles);
+      total += static_cast<long long>(pairs) * tiles;
     }
-    int sum = n;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += o;
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    const long long even = (total * a.groups + a.cut - 1) / a.cut;
+    most = clamp_to(even, 2 * a.min_tiles, 0x7fffffff);
+  }
+  long long before = 0;  // pieces of the sequences before
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    look(b0 + lane, &s, &pairs, &tiles);
+    const int parts = (tiles - 1) / most + 1;
+    const long long count = static_cast<long long>(pairs) * a.groups * parts;
+    long long first = before, all = 0;
+    for (int o = 0; o < 32; ++o) {
+      const long long c = __shfl_sync(0xffffffffu, count, o);
+      const int t = __shfl_sync(0xffffffffu, tiles, o);
+      if (t > tiles || (t == tiles && o < lane)) first += c;
+      all += c;
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, sum > idx);
-    if (past != 0) {
-      const int l = __ffs(past) - 1;
-      const int n_l = __shfl_sync(0xffffffffu, n, l), before = __shfl_sync(0xffffffffu, sum, l) - n_l;
-      r0 = __shfl_sync(0xffffffffu, r0, l);
-      r1 = __shfl_sync(0xffffffffu, r1, l);
-      *b = b0 + l;
-      *pair = n_l - 1 - (idx - before);  // the latest first: it sees the most keys
-      *s = cache_seq(a, r0, r1, a.seq_lens[b0 + l]);
+    const uint32_t mine = __ballot_sync(0xffffffffu, x >= first && x < first + count);
+    if (mine != 0) {
+      const int l = __ffs(mine) - 1;
+      it->b = b0 + l;
+      const int at = static_cast<int>(x - __shfl_sync(0xffffffffu, first, l));
+      it->n_parts = __shfl_sync(0xffffffffu, parts, l);
+      const int idx = at / it->n_parts;
+      it->part = at - idx * it->n_parts;
+      const int back = div_by(idx, a.by_groups);
+      it->group = idx - back * a.groups;
+      *pair = __shfl_sync(0xffffffffu, pairs, l) - 1 - back;  // the latest first: it sees the most keys
+      it->s = cache_seq(a, a.cu_q[it->b], a.cu_q[it->b + 1], a.seq_lens[it->b]);
       return true;
     }
-    idx -= __shfl_sync(0xffffffffu, sum, 31);
+    before += all;
   }
   return false;
 }
@@ -221,15 +247,20 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     grid_dep_wait();
 
     WsItem it{};
-    const int x = static_cast<int>(blockIdx.x);
-    const int idx = div_by(x, a.by_groups);
-    it.group = x - idx * a.groups;
-    it.item = x;
-    int pair;
+    int x = static_cast<int>(blockIdx.x), pair, single = -1;
     bool there = true;
     if (PREFIX || a.cu_q == nullptr) {
+      if (x >= a.pair_items) {  // the last wave's pairs, a Q tile to a CTA
+        single = (x - a.pair_items) & 1;
+        x = a.pair_items + ((x - a.pair_items) >> 1);
+      }
+      const int idx = div_by(x, a.by_groups);
+      it.group = x - idx * a.groups;
       it.b = PREFIX ? 0 : div_by(idx, a.by_pairs);
       pair = a.pairs - 1 - (idx - it.b * a.pairs);
+      it.part = static_cast<int>(blockIdx.y);
+      it.n_parts = static_cast<int>(gridDim.y);
+      it.slot0 = x * static_cast<int>(gridDim.y);
       if constexpr (PREFIX) {
         it.s.nq = a.cu_q != nullptr ? a.total_q : a.B * a.Nq;
         it.s.hi = clamp_to(a.shared, 0, static_cast<long long>(a.table_width) << a.page_shift);
@@ -237,25 +268,25 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         it.s = cache_seq(a, 0, 0, a.seq_lens != nullptr ? a.seq_lens[it.b] : 0);
       }
     } else {
-      there = ragged_pair(a, idx, &it.b, &pair, &it.s);
+      there = ragged_item(a, x, &it, &pair);
+      it.slot0 = x - it.part;
     }
     if (there) {
       if (it.s.bad && lane == 0 && a.status != nullptr) atomicOr(a.status, kErrCache);
-      it.q0 = pair * 2 * tpt;
-      it.nt = it.q0 + tpt < it.s.nq ? 2 : 1;
+      it.q0 = (pair * 2 + (single > 0 ? 1 : 0)) * tpt;
+      it.nt = it.q0 >= it.s.nq ? 0 : single < 0 && it.q0 + tpt < it.s.nq ? 2 : 1;
       // keys that rows of these tiles see
       int lo = it.s.lo, hi = it.s.hi, sink_end = it.s.sink_end;
       if constexpr (!PREFIX) {
         int first, end;
         cache_row(a, it.s, it.q0, &lo, &end);
-        cache_row(a, it.s, min(it.q0 + it.nt * tpt, it.s.nq) - 1, &first, &hi);
+        cache_row(a, it.s, max(min(it.q0 + it.nt * tpt, it.s.nq) - 1, 0), &first, &hi);
         lo = min(max(lo, it.s.lo), hi);
         sink_end = a.window > 0 ? min(a.sinks, lo) : 0;
       }
       it.t = cache_tiles<kTileN>(lo, hi, sink_end);
       if (lo >= hi && sink_end == 0) it.t.n = 0;
-      it.n_parts = max(1, min(static_cast<int>(gridDim.y), it.t.n / a.min_tiles));
-      it.part = static_cast<int>(blockIdx.y);
+      it.n_parts = max(1, min(it.n_parts, it.t.n / a.min_tiles));
       if (it.part >= it.n_parts) {
         it.nt = 0;
       } else {
@@ -479,7 +510,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       bool write_out = !PREFIX;
       float m_tot = m_cur, l_tot = l_run;
       // slots of the item's pieces: [piece][tile][D / 4][128 rows][4] floats, a warp stores 512 bytes in a row
-      const long long slot0 = static_cast<long long>(it.item) * gridDim.y * 2 + t;
+      const long long slot0 = static_cast<long long>(it.slot0) * 2 + t;
       if (PREFIX || it.n_parts > 1) {
         const long long my = (slot0 + 2 * it.part) * kTileM;
         a.part_ml[my + r] = make_float2(m_cur, l_run);
@@ -499,7 +530,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         named_bar_sync(1 + t, 128);
         if (r == 0) {
           __threadfence();
-          int* cnt = a.counters + 2 * it.item + t;
+          int* cnt = a.counters + 2 * it.slot0 + t;
           const int order = atomicAdd(cnt, 1);
           if (order == it.n_parts - 1) *cnt = 0;
           arrival[t] = order;
@@ -787,12 +818,12 @@ cache_merge_kernel(const CacheArgs a, int n_parts) {
 }
 
 template <int D, bool BF16, bool PREFIX, bool NARROW = false>
-static cudaError_t launch_t(const CUtensorMap* tm, const CacheArgs& a, int items, int parts, cudaStream_t st) {
+static cudaError_t launch_t(const CUtensorMap* tm, const CacheArgs& a, int ctas, int parts, cudaStream_t st) {
   auto kern = fwd_cache_ws_kernel<D, BF16, PREFIX, NARROW>;
   static std::atomic<unsigned long long> smem_set{0};
   cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(kern), Layout<D>::kDynSmem, &smem_set);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(kern, dim3(items, parts), kThreads, Layout<D>::kDynSmem, st, tm[0], tm[1], tm[2], tm[3], a);
+  return launch_overlapped(kern, dim3(ctas, parts), kThreads, Layout<D>::kDynSmem, st, tm[0], tm[1], tm[2], tm[3], a);
 }
 
 template <int D, bool BF16>
@@ -805,7 +836,8 @@ static cudaError_t launch_d(bool prefix, const CUtensorMap* tm, const CacheArgs&
 }
 
 // tm: Q (5-D, boxes of tpt tokens x pack heads), K, V (boxes of 64 columns x min(128, page size) keys), O (5-D, boxes of a
-// warp's 32 rows).  `items` pairs of Q tiles x groups of heads, each cut into at most `parts` pieces.
+// warp's 32 rows).  a.pair_items pairs of Q tiles x groups of heads, the rest of the `ctas` a Q tile each, all cut into at most
+// `parts` pieces; ragged: as many CTAs as there may be pieces.
 cudaError_t launch_fwd_cache_ws(int D, bool bf16, bool prefix, const CUtensorMap* tm, const CacheArgs& a, int items, int parts,
                                 cudaStream_t st) {
   if (D == 128)
