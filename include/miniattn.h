@@ -312,8 +312,8 @@ int miniattn_linear(const MiniAttnLinearParams* p, void* stream);
  * cu_q: the rows of sequence b are cu_q[b] .. cu_q[b + 1] - 1 of q, total_q rows in all; rows behind the last sequence's are
  * left as they are.  Null: Nq rows each.
  *
- * shared_len: the first shared_len tokens of all sequences are the same, in the pages that sequence 0 names; their keys are
- * read once for all.  A multiple of page_size; not with a window.
+ * shared_len: the first shared_len tokens of all sequences are the same, the rows of the block table begin with the same
+ * pages; their keys are read once for all where that is quicker.  A multiple of page_size; not with a window.
  *
  * A length, row number or page outside the call's tensors sets bit 7 of the status word; nothing outside them is read or
  * written, and the sequence's results are undefined, the others' are not.

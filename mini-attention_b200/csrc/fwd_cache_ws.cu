@@ -27,9 +27,9 @@ constexpr int kThreads = 384;
 constexpr int kWarpMma0 = 8, kWarpTma = 9, kWarpMma1 = 10, kWarpV = 11;
 constexpr int kHalfN = kTileN / 2;   // keys per half tile
 constexpr float kSumLimit = 256.0f;  // a half's sum of P above which the row's reference moves
-// registers per thread after setmaxnreg: 8 * 216 + 4 * 72 = 12 * 168, what the launch allocates
-constexpr int kRegSoftmax = 216;
-constexpr int kRegOther = 72;
+// registers per thread after setmaxnreg: 8 * 208 + 4 * 88 = 12 * 168, what the launch allocates
+constexpr int kRegSoftmax = 208;
+constexpr int kRegOther = 88;
 
 template <int D>
 struct Layout {
@@ -195,8 +195,7 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
 
 }  // namespace
 
-// PREFIX: the rows are those of all sequences, one after the other, the keys the a.shared first tokens of sequence 0's block
-// table; every piece is left for cache_merge_kernel, nothing is written to o.
+// PREFIX: the rows are those of all sequences, one after the other, the keys the a.shared first tokens of them; every piece is left for cache_merge_kernel, nothing is written to o.
 // NARROW: head dim 96 on the D = 128 tiles, the MMAs leave the 32 columns of zeros out.
 template <int D, bool BF16, bool PREFIX, bool NARROW>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -263,7 +262,15 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       it.slot0 = x * static_cast<int>(gridDim.y);
       if constexpr (PREFIX) {
         it.s.nq = a.cu_q != nullptr ? a.total_q : a.B * a.Nq;
-        it.s.hi = clamp_to(a.shared, 0, static_cast<long long>(a.table_width) << a.page_shift);
+        // read through the block table of the longest sequence: others may be padding, or end before the prefix does
+        int longest = -1;
+        for (int b = lane; b < a.B; b += 32) longest = max(longest, a.seq_lens[b]);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        int of = 0x7fffffff;
+        for (int b = lane; b < a.B; b += 32)
+          if (a.seq_lens[b] == longest) of = min(of, b);
+        it.b = __reduce_min_sync(0xffffffffu, of);
+        it.s.hi = clamp_to(min(a.shared, longest), 0, static_cast<long long>(a.table_width) << a.page_shift);
       } else {
         it.s = cache_seq(a, 0, 0, a.seq_lens != nullptr ? a.seq_lens[it.b] : 0);
       }
@@ -286,7 +293,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       }
       it.t = cache_tiles<kTileN>(lo, hi, sink_end);
       if (lo >= hi && sink_end == 0) it.t.n = 0;
-      it.n_parts = max(1, min(it.n_parts, it.t.n / a.min_tiles));
+      if (!PREFIX) it.n_parts = max(1, min(it.n_parts, it.t.n / a.min_tiles));  // a prefix's pieces are all added up
       if (it.part >= it.n_parts) {
         it.nt = 0;
       } else {

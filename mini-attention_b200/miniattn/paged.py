@@ -244,7 +244,7 @@ def paged_attention(
 
     ``max_q``, with ``cu_q``: the most rows that one sequence has.  It picks the kernel and nothing else; without it the rows
     of ``q`` are taken for it.  ``shared_len``: the first ``shared_len`` tokens (whole pages) are the same for all sequences,
-    in the pages that the first row of the block table names; they are read once for the whole batch.
+    the rows of the block table begin with the same pages; they are read once for the whole batch where that is quicker.
 
     Returns ``out`` or ``(out, lse)``, lse fp32, the natural logarithm of the softmax denominators: (B, Hq, n), or (Hq, rows)
     with ``cu_q``.  A NaN or infinity among the values of a key that any row of a sequence sees may show in others of its rows.

@@ -92,6 +92,44 @@ def test_shared_prefix(n, shared, page, D, dtype):
     _compare(p, _queries(p.news, 8, D, dtype), False, shared_len=shared)
 
 
+@pytest.mark.parametrize("dtype,D,n,Hkv,G", [(BF16, 128, 1, 8, 4), (F16, 64, 4, 16, 4), (BF16, 96, 2, 8, 3), (BF16, 128, 2, 2, 40)])
+def test_shared_prefix_of_a_batch(dtype, D, n, Hkv, G):
+    """Enough to be read in a launch of its own: 48 sequences, the first of them padding with nothing in its block table, some
+    shorter than the prefix."""
+    shared = 1024
+    lens = [0, n, 700, 1] + [shared + n + 29 * i for i in range(44)]
+    p = Paged(lens, [n] * len(lens), Hkv, D, dtype, 32, shared=shared, seed=D)
+    _compare(p, _queries(p.news, Hkv * G, D, dtype), False, shared_len=shared)
+
+
+def test_shared_prefix_longer_than_every_sequence():
+    lens = [0] + [900 - i for i in range(63)]
+    p = Paged(lens, [1] * 64, 8, 128, BF16, 16, shared=2048, seed=8)
+    table = torch.full((64, 200), 10 ** 6, dtype=torch.int32, device=DEV)  # nothing past the sequences' ends
+    table[:, :p.table.shape[1]] = p.table
+    p.table = table
+    _compare(p, _queries(p.news, 32, 128, BF16), False, shared_len=2048)
+
+
+def test_shared_prefix_ragged_batch():
+    """Ragged rows behind a prefix of a launch of its own, rows behind the last sequence, an empty sequence."""
+    shared = 2048
+    news = [1, 0, 4, 3, 2, 1, 4, 1] * 6
+    lens = [shared + 40 * i + m for i, m in enumerate(news)]
+    p = Paged(lens, news, 8, 128, BF16, 64, shared=shared, seed=9)
+    rows = _queries(news, 32, 128, BF16)
+    q = torch.cat(rows + [torch.full((5, 32, 128), float("nan"), dtype=BF16)]).to(DEV)
+    out = torch.full_like(q, 5.0)
+    _, lse = miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, cu_q=p.cu_q, max_q=4, shared_len=shared,
+                                      out=out, return_lse=True)
+    T = sum(news)
+    for b, (o, t, z, tz) in enumerate(zip(*p.expected(rows))):
+        check(out[:T].split(news)[b], o, t, f"sequence {b}")
+        check(lse[:, :T].split(news, 1)[b], z, tz, f"lse of sequence {b}")
+    assert bool((out[T:] == 5).all())
+    miniattn.check_device_status(DEV)
+
+
 def test_shared_prefix_ragged():
     shared = 512
     news = [1, 0, 200, 3, 65, 1]
