@@ -1080,7 +1080,8 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
     c.rg = rows <= 16 ? 1 : 2;
     c.n_ctas = 2 * sms;
     c.part_rows = static_cast<size_t>(2 * c.n_ctas) * 16 * c.rg;
-    const bool stacked = ragged || p->Nq == 1 || p->q_stride[0] == p->Nq * p->q_stride[2];
+    // the rows of all sequences at one distance
+    const bool stacked = ragged || (p->Nq == 1 ? p->q_stride[0] >= p->D || p->B == 1 : p->q_stride[0] == p->Nq * p->q_stride[2]);
     const long long all = ragged ? p->total_q : static_cast<long long>(p->B) * p->Nq, pairs = (all + span - 1) / span;
     // What all sequences would read of it without: the two launches more and the pieces between them cost about as much as
     // 100 MB of it.  With and without, 32/8 heads of 128: 16 x 1024 tokens (67 MB) 21.5 / 17.5 us, 64 x 512 (134) 29.0 / 28.8,

@@ -6,13 +6,20 @@
 //
 //   item      = (sequence, KV head, block of 16 * RG rows); a row is (token, query head of the KV head's G), so that K and V
 //               cross an SM once for all the heads that share them
-//   CTA       = a contiguous range of the 64-key tiles of all items, the same length for each: lengths are known on the GPU
-//               alone, so every CTA adds up the tiles of all sequences and finds its own
+//   CTA       = a contiguous range of the 64-key tiles of all items, the same length for each (an item counts kItemCost tiles
+//               more: dealt out by tiles alone, 512 items of 1 to 16 tiles took 44 instead of 26 us); lengths are known on the
+//               GPU alone, so every CTA adds up the tiles of all sequences and finds its own
 //   warp 4    TMA producer: a copy per page (at most 64 keys) and 64 columns of K and of V, each issued by a lane of its own
 //   warps 0-3 16 rows x (16 * RG keys of the tile) each, running (m, l, O) in registers
 //
 // A CTA whose range cuts an item leaves its piece (un-normalised O, m, l) in scratch and counts itself in; the one that
 // counts in last folds the pieces.  Behind a shared prefix the rows are left un-normalised for the launch that adds its pieces.
+//
+// Bound: HBM where the contexts are long: 16 requests of 1001 to 16001 keys, 32/8 heads of 128, pages of 16 tokens 67 us = 5.6
+// TB/s, 0.86 of the measured copy rate; 32 with a window of 4096 87 us = 6.0 TB/s.  Short calls are bound by their chain of
+// loads: lengths (0.7 us), the walk to the CTA's range (0.8), block table and first tile (1.2), half a microsecond a tile, 0.5
+// to leave a piece and 3 to fold: 4 requests of 100 to 1000 keys, 12 heads of 64 9 us (pieces of 4 tiles; of 6, 8 and 12: 9.5,
+// 10.1, 11.9).
 //
 // Keys that no row sees are never read: their pages may be gone or hold anything.  Where a tile holds some, their scores
 // are replaced and their rows of V cleared, so that what lies there does not reach a result.
@@ -21,6 +28,7 @@
 
 #include "cache.cuh"
 #include "launch.cuh"
+#include "mma_sync.cuh"
 #include "ptx.cuh"
 
 namespace ma {
@@ -50,25 +58,6 @@ struct Layout {
   static constexpr int kDynSmem = kBytes + 1024;
 };
 
-__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // weight of a partial with maximum m under the total maximum mt (0 for a partial without keys)
@@ -217,7 +206,8 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   auto next_seq = [&]() {  // the next sequence that has rows; only while places are left
     do {
       base += w.total(a);
-      w = walk_to<kRows>(a, ++b, pieces);
+      b = min(b + 1, a.B - 1);
+      w = walk_to<kRows>(a, b, pieces);
     } while (w.n_rb == 0 && b + 1 < a.B);
   };
 
@@ -305,7 +295,7 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   int slot = 0, par = 0;
 
   for (long long x = lo; x < hi;) {
-    while (x >= base + w.total(a)) next_seq();
+    while (x >= base + w.total(a) && b + 1 < a.B) next_seq();
     const long long it = cache_div(x - base, w.slots);
     const long long item0 = base + it * w.slots;
     const int t0 = static_cast<int>(x - item0);
@@ -315,6 +305,7 @@ fwd_cache_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       continue;
     }
     const int hk = static_cast<int>(cache_div(it, w.n_rb)), rb = static_cast<int>(it - static_cast<long long>(hk) * w.n_rb);
+    if (hk >= a.Hkv) break;  // only if the lengths changed under the launch
     const int rows = w.s.nq * a.G, row0 = rb * kRows;
 
     // Q fragments of this warp's 16 rows, and which keys its two rows of this lane see
@@ -668,8 +659,7 @@ static cudaError_t launch_t(const CUtensorMap* tm, const CacheArgs& a, int n_cta
 template <int D, bool BF16>
 static cudaError_t launch_d(const CUtensorMap* tm, const CacheArgs& a, int rg, int n_ctas, cudaStream_t st) {
   if (rg == 1) return launch_t<D, BF16, 1>(tm, a, n_ctas, st);
-  if (rg == 2) return launch_t<D, BF16, 2>(tm, a, n_ctas, st);
-  return launch_t<D, BF16, 4>(tm, a, n_ctas, st);
+  return launch_t<D, BF16, 2>(tm, a, n_ctas, st);
 }
 
 // tm[0], tm[1]: K and V maps with boxes of 64 columns x min(64, page size) keys.

@@ -13,6 +13,18 @@
 //
 // Tiles at the ends hold keys that no row of the sequence sees and that may be anything.  Their scores are replaced; their
 // rows of V are cleared in shared memory by warp 11, which hands such a tile over itself instead of leaving that to the copy.
+//
+// Bound: tensor pipe and power where items are long (16384 tokens, 32/8 heads of 128, window 4096, 4 sinks 860 us = 1.1 PFLOP/s;
+// 1.7 us a 128-key step of a CTA at the power cap).  Short windows are bound by a CTA's ends and by the tiles that only some of
+// its 256 rows see: 4 x 1024 tokens, 12 heads of 64, window 256 20.6 us, 3 us of an item's 12 outside its steps.
+//
+// The query heads of a KV head always share Q tiles: a pair of tiles then spans 256 / G tokens, and its band of keys is that
+// much narrower.
+//
+// Built and dropped: one CTA an SM that walks a contiguous part of all items' tiles (cut evenly, no second wave).  Its start
+// takes 4.5 us instead of 1.5, and without the offset that each item gives its second Q tile the two softmax groups fall into
+// step, in which a 64-key half takes 1750 clk instead of 1520: 860 -> 985 us, 20.6 -> 24 us; only mixed chunks gained.  Turns
+// that keep the groups apart, through a barrier between the MMA warps, cost more than the step (2000 clk).
 #include <atomic>
 
 #include "cache.cuh"
@@ -68,21 +80,6 @@ struct WsItem {
 };
 static_assert(sizeof(WsItem) <= 96, "WsItem");
 
-__device__ __forceinline__ void named_bar_sync(int id, int n) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void reg_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void reg_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-__device__ __forceinline__ void warp_arrive(uint32_t bar) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
 __device__ __forceinline__ float part_weight(float m, float mt) { return m == -INFINITY ? 0.f : ex2(m - mt); }
 __device__ __forceinline__ float row_lse(float m, float l) {
   return l == 0.f ? -INFINITY : m * 0.6931471805599453f + __logf(l);
