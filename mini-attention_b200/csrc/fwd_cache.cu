@@ -7,7 +7,7 @@
 //   item      = (sequence, KV head, block of 16 * RG rows); a row is (token, query head of the KV head's G), so that K and V
 //               cross an SM once for all the heads that share them
 //   CTA       = a contiguous range of the 64-key tiles of all items, the same length for each (an item counts kItemCost tiles
-//               more: dealt out by tiles alone, 512 items of 1 to 16 tiles took 44 instead of 26 us); lengths are known on the
+//               more: dealt out by tiles alone, 512 items of 1 to 16 tiles took 26.5 instead of 21.3 us, cold); lengths are known on the
 //               GPU alone, so every CTA adds up the tiles of all sequences and finds its own
 //   warp 4    TMA producer: a copy per page (at most 64 keys) and 64 columns of K and of V, each issued by a lane of its own
 //   warps 0-3 16 rows x (16 * RG keys of the tile) each, running (m, l, O) in registers
@@ -19,7 +19,7 @@
 // TB/s, 0.86 of the measured copy rate; 32 with a window of 4096 87 us = 6.0 TB/s.  Short calls are bound by their chain of
 // loads: lengths (0.7 us), the walk to the CTA's range (0.8), block table and first tile (1.2), half a microsecond a tile, 0.5
 // to leave a piece and 3 to fold: 4 requests of 100 to 1000 keys, 12 heads of 64 9 us (pieces of 4 tiles; of 6, 8 and 12: 9.5,
-// 10.1, 11.9).
+// 10.1, 11.9, with an earlier fold).
 //
 // Keys that no row sees are never read: their pages may be gone or hold anything.  Where a tile holds some, their scores
 // are replaced and their rows of V cleared, so that what lies there does not reach a result.

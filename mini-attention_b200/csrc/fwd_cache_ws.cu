@@ -23,7 +23,7 @@
 //
 // Built and dropped: one CTA an SM that walks a contiguous part of all items' tiles (cut evenly, no second wave).  Its start
 // takes 4.5 us instead of 1.5, and without the offset that each item gives its second Q tile the two softmax groups fall into
-// step, in which a 64-key half takes 1750 clk instead of 1520: 860 -> 985 us, 20.6 -> 24 us; only mixed chunks gained.  Turns
+// step, in which a 64-key half takes 1750 clk instead of 1520: both calls above took 14 % longer, only mixed chunks gained.  Turns
 // that keep the groups apart, through a barrier between the MMA warps, cost more than the step (2000 clk).
 #include <atomic>
 
