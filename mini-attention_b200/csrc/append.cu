@@ -74,7 +74,7 @@ append_kernel(const AppendArgs a) {
     long long first, n_new;
     if (a.cu_q != nullptr) {
       b = sequence_of(a, t);
-      if (b >= a.B) continue;  // rows behind the last sequence are left as they are
+      if (b >= a.B) continue;  // behind the last sequence's rows
       first = a.cu_q[b];
       n_new = a.cu_q[b + 1] - first;
     } else {
@@ -85,7 +85,7 @@ append_kernel(const AppendArgs a) {
     const AppendSlot s = append_slot(a, t, first, n_new, a.seq_lens[b],
                                      [&](int i) { return a.table[b * a.table_stride + i]; });
     if (s.bad && tid == 0 && a.status != nullptr) atomicOr(a.status, kErrCache);
-    if (tid >= lanes) continue;
+    if (s.none || tid >= lanes) continue;
     float cs[8], sn[8];
     const bool turn = turns && s.held;
     if (turn) {

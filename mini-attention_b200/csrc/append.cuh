@@ -23,10 +23,11 @@ struct AppendArgs {
   FastDiv by_n, by_units;
 };
 
-// Sequence and position of row t.  False: the row belongs to no sequence, or its position lies before the sequence's first.
+// Where row t of a sequence goes.
 struct AppendSlot {
-  bool held;            // the cache has a place for it
-  bool bad;             // a length, a page or a position outside the call's tensors
+  bool none;            // the row belongs to no sequence: it is left as it is, and so is its query
+  bool held;            // the cache has a place for it (not for one before the sequence's first token)
+  bool bad;             // a length, a row, a page or a position outside the call's tensors
   int pos;
   long long page;       // page and token of the page, where held
   int at;
@@ -36,9 +37,18 @@ template <typename Table>
 __host__ __device__ inline AppendSlot append_slot(const AppendArgs& a, int t, long long first, long long n_new, int seq_len,
                                                   const Table& table) {
   AppendSlot s{};
+  const bool rows_bad = first < 0 || first + n_new > a.rows || t >= first + n_new;  // the last where row numbers fall
+  if (t < first || rows_bad) {  // before the first sequence's rows
+    s.none = true;
+    s.bad = rows_bad;
+    return s;
+  }
   const long long pos = seq_len - n_new + (t - first);
   const long long room = static_cast<long long>(a.table_width) << a.page_shift;
-  if (pos < 0) return s;  // the front of a padded sequence
+  if (pos < 0) {  // the front of a padded sequence
+    s.bad = seq_len < 0;
+    return s;
+  }
   if (pos >= room || (a.rope != nullptr && pos >= a.rope_rows)) {
     s.bad = true;
     return s;

@@ -105,6 +105,32 @@ def test_in_place_and_rows_behind():
     assert torch.equal(q[:20], apart[:20]) and torch.equal(q[20:], behind) and bool((apart[20:] == 3).all())
 
 
+def test_rows_in_front_of_the_first_sequence():
+    """They belong to no sequence: nothing of the cache is written for them, their queries stay."""
+    rope = miniattn.rope_table(64, 64, device=DEV)
+    k, v, q = _new([12], 4, 2, 64, BF16)
+    got = []
+    for skip in (0, 5):
+        caches, table, seq_lens = _setup([9, 30], 16, 2, 64, BF16)
+        cu = torch.tensor([5 - skip, 8 - skip, 12 - skip], dtype=torch.int32, device=DEV)
+        out = torch.full_like(q[skip:], 3.0)
+        miniattn.paged_append(k[skip:], v[skip:], *caches, table, seq_lens, cu_q=cu, q=q[skip:], q_out=out, rope=rope)
+        got.append((*caches, out[5 - skip:]))
+        assert bool((out[:5 - skip] == 3).all())
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    miniattn.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("cu,lens", [([-2, 4, 8], [9, 30]), ([0, 4, 40], [9, 30]), ([0, 6, 2], [9, 30]), ([0, 4, 8], [9, -1])])
+def test_bad_rows_and_negative_lengths_are_reported(cu, lens):
+    caches, table, _ = _setup([9, 30], 16, 2, 64, BF16)
+    k, v, q = _new([8], 4, 2, 64, BF16)
+    cu, lens = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (cu, lens))
+    miniattn.paged_append(k, v, *caches, table, lens, cu_q=cu, q=q)
+    with pytest.raises(RuntimeError, match="outside its tensors"):
+        miniattn.check_device_status(DEV)
+
+
 def test_far_positions():
     """A table made in 64 bits: position 10^6 is rotated as exactly as position 0."""
     rope = miniattn.rope_table(1_000_001, 128, theta=500.0, device=DEV)

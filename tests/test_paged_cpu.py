@@ -239,16 +239,21 @@ int main() {
     a.rope_rows = std::rand() % 600;
     const long long first = std::rand() % 50, n_new = std::rand() % 50;
     const int t = std::rand() % 100;
+    a.rows = std::rand() % 8 ? 100 : std::rand() % 100;
     int len = std::rand() % 700;
     if (std::rand() % 8 == 0) len = std::rand() % 2 ? -std::rand() : 2147483647 - std::rand() % 3;
     const int page = std::rand() % 8 - 2;
     int asked = -1;
     const AppendSlot s = append_slot(a, t, first, n_new, len, [&](int i) { asked = i; return page; });
+    const bool rows_bad = first + n_new > a.rows || t >= first + n_new;
+    if (s.none != (t < first || rows_bad)) return 5;
+    if (s.none && (s.held || asked != -1 || s.bad != rows_bad)) return 6;
+    if (s.none) continue;
     const long long pos = len - n_new + (t - first);
     if (asked >= a.table_width) return 1;                                    // outside the block table
     const bool room = pos >= 0 && pos < ((long long)a.table_width << a.page_shift) && (!a.rope || pos < a.rope_rows);
     if (s.held != (room && page >= 0 && page < a.n_pages)) return 2;
-    if (s.bad != (pos >= 0 && !s.held)) return 3;
+    if (s.bad != (pos >= 0 ? !s.held : len < 0)) return 3;
     if (s.held && (s.pos != pos || s.page != page || s.at != (pos & ((1 << a.page_shift) - 1)) || asked != (pos >> a.page_shift))) return 4;
   }
   std::printf("ok\n");
