@@ -82,7 +82,7 @@ __host__ __device__ inline CacheSeq cache_seq(const CacheArgs& a, int first_row,
   s.diag = a.diag;
   if (a.seq_lens != nullptr) {
     const long long room = static_cast<long long>(a.table_width) << a.page_shift;
-    len = clamp_to(seq_len, 0, room < 0x7fffffc0ll ? room : 0x7fffffc0ll);
+    len = clamp_to(seq_len, 0, room < 0x7fffff00ll ? room : 0x7fffff00ll);  // rounded up to tiles it fits in 31 bits
     s.bad = s.bad || len != seq_len;
     s.diag = len - s.nq;
   }

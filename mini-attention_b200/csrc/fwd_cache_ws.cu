@@ -149,15 +149,21 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
   CacheSeq s{};
   int pairs, tiles, most = 0x7fffffff;  // tiles of a piece
   if (a.cut > 0) {
-    long long total = 0;
+    long long total = 0, items = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       look(b0 + lane, &s, &pairs, &tiles);
       total += static_cast<long long>(pairs) * tiles;
+      items += pairs;
     }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    for (int d = 16; d > 0; d >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, d);
+      items += __shfl_xor_sync(0xffffffffu, items, d);
+    }
     const long long even = (total * a.groups + a.cut - 1) / a.cut;
-    most = clamp_to(even, 2 * a.min_tiles, 0x7fffffff);
+    // Rows that overlap, which only row numbers that fall give, may be more than the launch has CTAs for: a piece without one
+    // would leave its item's counter standing, so nothing is cut then.
+    if (items * a.groups + a.cut <= gridDim.x) most = clamp_to(even, 2 * a.min_tiles, 0x7fffffff);
   }
   long long before = 0;  // pieces of the sequences before
   for (int b0 = 0; b0 < a.B; b0 += 32) {

@@ -12,11 +12,11 @@ later steps as well.  The conventions both share:
 * ``seq_lens``: (B,) int32, the tokens of each sequence, the new ones among them and last: new token i of n sits at position
   ``seq_lens[b] - n + i``.  A sequence of length 0 takes no part: its rows of the result are 0.
 * New tokens come as (B, n, heads, D), or ragged as (rows, heads, D) with ``cu_q``, (B + 1,) int32: the rows of sequence b are
-  ``cu_q[b]`` to ``cu_q[b + 1] - 1``.  Rows behind the last sequence's are left as they are.
+  ``cu_q[b]`` to ``cu_q[b + 1] - 1``.  Rows before the first sequence's and behind the last one's are left as they are.
 
 A length, row, page or position outside these tensors is found on the device: it sets a bit that
 :func:`miniattn.check_device_status` turns into an error, nothing outside them is read or written, and that sequence's results
-are undefined.
+are undefined.  The tensors must not change while a call runs.
 """
 from __future__ import annotations
 
@@ -149,9 +149,9 @@ def paged_append(
 
     With ``rope`` (a table of :func:`rope_table`, its width the rotated part of each head, a multiple of 16) the keys are
     rotated by their positions on the way, and so is ``q``, the queries of the same tokens, which come back in ``q_out``
-    (a new tensor by default; ``q`` itself is fine).  Pairs are elements (i, i + width / 2) of a head, neighbours
-    (2 i, 2 i + 1) with ``interleaved``.  Tokens at negative positions (the front of a padded sequence, ``seq_lens[b] < n``) are
-    left out and their queries copied.  Two tokens of one call must not go to the same place of the cache, which a block
+    (a new tensor by default; ``q`` itself is fine, any other overlap is not).  Pairs are elements (i, i + width / 2) of a
+    head, neighbours (2 i, 2 i + 1) with ``interleaved``.  Tokens at negative positions (the front of a padded sequence,
+    ``seq_lens[b] < n``) are left out and their queries copied.  Two tokens of one call must not go to the same place of the cache, which a block
     table that gives a page to one writing sequence at a time ensures.
 
     Returns the rotated queries, or None without ``q``.

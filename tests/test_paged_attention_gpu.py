@@ -173,6 +173,52 @@ def test_cache_layouts_and_strides():
     assert bool((out[:, :, 8] == 7).all())
 
 
+@pytest.mark.parametrize("lens,n,G,shared", [([3000, 1700], 1, 4, 0), ([3000, 1700], 40, 4, 0), ([900, 700], 200, 1, 0),
+                                             ([1100 + 17 * i for i in range(48)], 1, 8, 1024)])
+def test_result_in_place_of_the_queries(lens, n, G, shared):
+    p = Paged(lens, [n] * len(lens), 4, 128, BF16, 32, seed=31, shared=shared)
+    rows = _queries(p.news, 4 * G, 128, BF16)
+    q = torch.stack(rows).to(DEV)
+    assert miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, shared_len=shared, out=q) is q
+    for b, (o, t, *_) in enumerate(zip(*p.expected(rows))):
+        check(q[b], o, t, f"sequence {b}")
+
+
+@pytest.mark.parametrize("n,G,D", [(1, 129, 64), (3, 129, 128), (20, 129, 128), (2, 200, 96)])
+def test_more_heads_than_a_tile_has_rows(n, G, D):
+    p = Paged([700, 41, 5], [n, n, n], 1, D, F16, 16, seed=32)
+    rows = _queries(p.news, G, D, F16)
+    out = miniattn.paged_attention(torch.stack(rows).to(DEV), p.k_cache, p.v_cache, p.table, p.seq_lens)
+    for b, (o, t, *_) in enumerate(zip(*p.expected(rows))):
+        check(out[b], o, t, f"sequence {b}")
+
+
+@pytest.mark.parametrize("most", [1, 5, 4000])
+def test_max_q_picks_the_kernel_alone(most):
+    """Also where it is not what it says it is."""
+    p = Paged([900, 1300, 64, 2000], [70, 1, 0, 300], 2, 64, BF16, 32, seed=33)
+    rows = _queries(p.news, 8, 64, BF16)
+    out, lse = miniattn.paged_attention(torch.cat(rows).to(DEV), p.k_cache, p.v_cache, p.table, p.seq_lens, cu_q=p.cu_q,
+                                        max_q=most, return_lse=True)
+    at = 0
+    for b, (o, t, z, tz) in enumerate(zip(*p.expected(rows))):
+        check(out[at:at + p.news[b]], o, t, f"sequence {b}")
+        check(lse[:, at:at + p.news[b]], z, tz, f"lse of sequence {b}")
+        at += p.news[b]
+
+
+@pytest.mark.parametrize("n", [1, 33])
+def test_queries_shared_by_the_batch(n):
+    """One sequence's queries expanded over the batch, a stride of 0."""
+    p = Paged([700, 300, 64], [n] * 3, 2, 128, BF16, 16, seed=34)
+    rows = _queries([n], 8, 128, BF16) * 3
+    q = rows[0].to(DEV).expand(3, n, 8, 128)
+    out = torch.empty((3, n, 8, 128), dtype=BF16, device=DEV)
+    miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, out=out)
+    for b, (o, t, *_) in enumerate(zip(*p.expected(rows))):
+        check(out[b], o, t, f"sequence {b}")
+
+
 def test_rows_behind_the_last_sequence_stay():
     p = Paged([40, 300], [3, 100], 2, 64, BF16, 16, seed=7)
     rows = _queries([3, 100], 4, 64, BF16)
@@ -201,21 +247,24 @@ def test_same_bits_again(n):
         assert all(torch.equal(x, y) for x, y in zip(first, again))
 
 
-def test_two_streams():
-    p = Paged([3000, 1700], [1, 1], 2, 128, BF16, 32, seed=9)
-    rows = _queries([1, 1], 8, 128, BF16)
+@pytest.mark.parametrize("lens,n,G,shared", [([3000, 1700], 1, 4, 0), ([3000, 1700], 40, 4, 0),
+                                             ([1100 + 17 * i for i in range(48)], 1, 8, 1024)])
+def test_two_streams(lens, n, G, shared):
+    p = Paged(lens, [n] * len(lens), 4, 128, BF16, 32, seed=9, shared=shared)
+    rows = _queries(p.news, 4 * G, 128, BF16)
     q = torch.stack(rows).to(DEV)
+    want = list(zip(*p.expected(rows)))
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
     outs = []
     for _ in range(10):
         for s in streams:
             with torch.cuda.stream(s):
-                outs.append(miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens))
+                outs.append(miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, shared_len=shared))
     torch.cuda.synchronize()
-    for out in outs:
-        for b, (o, t, *_) in enumerate(zip(*p.expected(rows))):
-            check(out[b], o, t, f"sequence {b}")
+    assert all(torch.equal(out, outs[0]) for out in outs)
+    for b, (o, t, *_) in enumerate(want):
+        check(outs[0][b], o, t, f"sequence {b}")
 
 
 def test_bad_lengths_and_pages_are_reported():
@@ -271,6 +320,53 @@ def test_captured_call_serves_longer_contexts():
                 o, t, *_ = attention(rows[b].to(DEV), whole.k[b][:step[b]].to(DEV), whole.v[b][:step[b]].to(DEV), step[b] - 1)
                 check(out[b], o, t, f"step {k}, sequence {b}")
     miniattn.check_device_status(DEV)
+
+
+def test_captured_ragged_call_serves_other_batches():
+    """One graph of a ragged call, replayed for batches of other rows and lengths (its grid knows the sizes of q alone)."""
+    from paged_reference import attention
+    whole = Paged([1500, 900, 2100, 64], [1, 1, 1, 1], 2, 128, BF16, 16, seed=21)
+    for b in range(4):  # every token of every sequence is there
+        for j in range(whole.lens[b]):
+            if int(whole.table[b, j // 16]) < whole.k_cache.shape[0]:
+                whole.k_cache[int(whole.table[b, j // 16]), j % 16] = whole.k[b][j].to(DEV)
+                whole.v_cache[int(whole.table[b, j // 16]), j % 16] = whole.v[b][j].to(DEV)
+    q = torch.zeros((300, 8, 128), dtype=BF16, device=DEV)
+    lens, cu = whole.seq_lens.clone(), torch.tensor([0, 1, 2, 3, 300], dtype=torch.int32, device=DEV)
+    miniattn.paged_attention(q, whole.k_cache, whole.v_cache, whole.table, lens, cu_q=cu)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = miniattn.paged_attention(q, whole.k_cache, whole.v_cache, whole.table, lens, cu_q=cu, return_lse=True)
+    for k, (news, now) in enumerate([([100, 0, 200, 0], [1500, 10, 2100, 0]), ([1, 290, 1, 8], [700, 900, 1, 64]),
+                                     ([0, 0, 0, 60], [0, 0, 0, 64]), ([75, 75, 75, 64], [75, 900, 80, 64])]):
+        rows = _queries(news, 8, 128, BF16, seed=k)
+        q[:sum(news)] = torch.cat(rows).to(DEV)
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        cu.copy_(torch.tensor([0] + list(torch.tensor(news).cumsum(0)), dtype=torch.int32))
+        g.replay()
+        at = 0
+        for b, n in enumerate(news):
+            o, t, z, tz = attention(rows[b].to(DEV), whole.k[b][:now[b]].to(DEV), whole.v[b][:now[b]].to(DEV), now[b] - n)
+            check(out[at:at + n], o, t, f"batch {k}, sequence {b}")
+            check(lse[:, at:at + n], z, tz, f"lse of batch {k}, sequence {b}")
+            at += n
+    miniattn.check_device_status(DEV)
+
+
+def test_row_numbers_that_fall_do_no_lasting_harm():
+    """Overlapping rows (cu_q falls) are reported; the calls after it are right."""
+    p = Paged([900, 900, 900, 900], [200, 200, 0, 0], 2, 128, BF16, 16, seed=22)
+    rows = _queries([200, 200], 8, 128, BF16)
+    q = torch.cat(rows).to(DEV)
+    bad = torch.tensor([0, 400, 0, 400, 0], dtype=torch.int32, device=DEV)
+    for _ in range(3):
+        miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, cu_q=bad)
+        out = miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, cu_q=p.cu_q)
+        for b, (o, t, *_) in enumerate(list(zip(*p.expected(rows + _queries([0, 0], 8, 128, BF16))))[:2]):
+            check(out.split(200)[b], o, t, f"sequence {b}")
+    with pytest.raises(RuntimeError, match="outside its tensors"):
+        miniattn.check_device_status(DEV)
 
 
 def test_far_into_a_large_cache():
