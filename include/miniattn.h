@@ -309,8 +309,8 @@ int miniattn_linear(const MiniAttnLinearParams* p, void* stream);
  * k and v are [n_pages, page_size, Hkv, D] with any (page, head, token) strides.  Entries whose keys no row sees are not
  * read, nor are those keys.  page_size 0: no pages, k and v are [B, Hkv, Nk, D], strides (batch, head, token).
  *
- * cu_q: the rows of sequence b are cu_q[b] .. cu_q[b + 1] - 1 of q, total_q rows in all; rows behind the last sequence's are
- * left as they are.  Null: Nq rows each.
+ * cu_q: the rows of sequence b are cu_q[b] .. cu_q[b + 1] - 1 of q, total_q rows in all; rows before the first sequence's and
+ * behind the last one's are left as they are.  Null: Nq rows each.
  *
  * shared_len: the first shared_len tokens of all sequences are the same, the rows of the block table begin with the same
  * pages; their keys are read once for all where that is quicker.  A multiple of page_size; not with a window.
@@ -363,8 +363,8 @@ int64_t miniattn_fwd_cache_scratch_bytes(const MiniAttnCacheParams* p);
  * rope: [rope_rows, rot] fp32, the cosines of the rot / 2 angles of each position and then their sines; null: nothing is
  * rotated.  Pairs are elements (i, i + rot / 2), with `interleaved` (2i, 2i + 1); elements from rot on stay as they are.
  * Tokens before position 0 (the front of a padded sequence) are left out, their rows of q copied.  A position past the block
- * table or the rotation table, or a page outside the cache, sets bit 7 of the status word; the token is left out.  Two tokens
- * of one call must not go to the same place.
+ * table or the rotation table, a page outside the cache, rows outside the call's or that fall, or a negative length set bit 7
+ * of the status word; the token is left out.  Two tokens of one call must not go to the same place.
  */
 typedef struct MiniAttnAppendParams {
   const void* k;

@@ -7,8 +7,8 @@
 //   item      = (sequence, KV head, block of 16 * RG rows); a row is (token, query head of the KV head's G), so that K and V
 //               cross an SM once for all the heads that share them
 //   CTA       = a contiguous range of the 64-key tiles of all items, the same length for each (an item counts kItemCost tiles
-//               more: dealt out by tiles alone, 512 items of 1 to 16 tiles took 26.5 instead of 21.3 us, cold); lengths are known on the
-//               GPU alone, so every CTA adds up the tiles of all sequences and finds its own
+//               more: dealt out by tiles alone, 512 items of 1 to 16 tiles took 26.5 instead of 21.3 us, cold); lengths are
+//               known on the GPU alone, so every CTA adds up the tiles of all sequences and finds its own
 //   warp 4    TMA producer: a copy per page (at most 64 keys) and 64 columns of K and of V, each issued by a lane of its own
 //   warps 0-3 16 rows x (16 * RG keys of the tile) each, running (m, l, O) in registers
 //

@@ -198,7 +198,8 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
 
 }  // namespace
 
-// PREFIX: the rows are those of all sequences, one after the other, the keys the a.shared first tokens of them; every piece is left for cache_merge_kernel, nothing is written to o.
+// PREFIX: the rows are those of all sequences, one after the other, the keys the a.shared first tokens of them; every piece is
+// left for cache_merge_kernel, nothing is written to o.
 // NARROW: head dim 96 on the D = 128 tiles, the MMAs leave the 32 columns of zeros out.
 template <int D, bool BF16, bool PREFIX, bool NARROW>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -839,8 +840,10 @@ static cudaError_t launch_t(const CUtensorMap* tm, const CacheArgs& a, int ctas,
 template <int D, bool BF16>
 static cudaError_t launch_d(bool prefix, const CUtensorMap* tm, const CacheArgs& a, int items, int parts, cudaStream_t st) {
   if constexpr (D == 128) {
-    if (a.D == 96)
-      return prefix ? launch_t<D, BF16, true, true>(tm, a, items, parts, st) : launch_t<D, BF16, false, true>(tm, a, items, parts, st);
+    if (a.D == 96) {
+      if (prefix) return launch_t<D, BF16, true, true>(tm, a, items, parts, st);
+      return launch_t<D, BF16, false, true>(tm, a, items, parts, st);
+    }
   }
   return prefix ? launch_t<D, BF16, true>(tm, a, items, parts, st) : launch_t<D, BF16, false>(tm, a, items, parts, st);
 }

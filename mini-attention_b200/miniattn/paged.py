@@ -151,8 +151,8 @@ def paged_append(
     rotated by their positions on the way, and so is ``q``, the queries of the same tokens, which come back in ``q_out``
     (a new tensor by default; ``q`` itself is fine, any other overlap is not).  Pairs are elements (i, i + width / 2) of a
     head, neighbours (2 i, 2 i + 1) with ``interleaved``.  Tokens at negative positions (the front of a padded sequence,
-    ``seq_lens[b] < n``) are left out and their queries copied.  Two tokens of one call must not go to the same place of the cache, which a block
-    table that gives a page to one writing sequence at a time ensures.
+    ``seq_lens[b] < n``) are left out and their queries copied.  Two tokens of one call must not go to the same place of the
+    cache, which a block table that gives a page to one writing sequence at a time ensures.
 
     Returns the rotated queries, or None without ``q``.
     """

@@ -126,8 +126,8 @@ class GQA_Flash(nn.Module):
         """New tokens x, (B, n, d_model) or (rows, d_model) with ``cu_q``, of sequences whose keys and values lie in pages: theirs
         are appended (``seq_lens`` counts them already) and they attend to everything their sequences hold, as
         :func:`miniattn.paged_append` and :func:`miniattn.paged_attention` say."""
-        return _serve(linear(x, self.w_q, self.kv), self.w_o, self.n_kv_heads, self.head_dim, k_cache, v_cache, block_table, seq_lens, cu_q,
-                      max_q, rope, interleaved, window, sinks, shared_len)
+        return _serve(linear(x, self.w_q, self.kv), self.w_o, self.n_kv_heads, self.head_dim, k_cache, v_cache, block_table,
+                      seq_lens, cu_q, max_q, rope, interleaved, window, sinks, shared_len)
 
 
 class MQA_Flash(nn.Module):
