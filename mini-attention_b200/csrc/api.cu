@@ -1092,7 +1092,8 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
       c.pre_pairs = static_cast<int>(pairs);
       c.pre_items = c.pre_pairs * c.groups;
       const int tiles = tiles_of(p->shared_len);
-      c.pre_parts = std::max(1, std::min(sms / c.pre_items, tiles / kMinPrefixTiles));
+      const int most = std::max(1, std::min(sms / c.pre_items, tiles / kMinPrefixTiles)), each = std::max(1, (tiles + most - 1) / most);
+      c.pre_parts = std::max(1, (tiles + each - 1) / each);  // as few as take no longer
       c.pre_rows = static_cast<size_t>(c.pre_items) * c.pre_parts * 2 * ma::kTileM;
       c.rest_rows = static_cast<size_t>(all) * p->Hq;
     }

@@ -766,55 +766,55 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 
 // ---------------------------------------------------------------------------------
 // The rows of a call behind a shared prefix: the pieces that the prefix's launch left and what the launch over the rest of
-// each sequence left, added up and stored.  A warp takes 32 rows of a Q tile and 8 columns of them, a lane a row.
+// each sequence left, added up and stored.  A warp takes 32 rows of a Q tile and 4 columns of them, a lane a row.  Bound: the
+// loads that wait for one another, so a running maximum instead of a pass over the pieces for it, and kAhead pieces together.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(128)
 cache_merge_kernel(const CacheArgs a, int n_parts) {
   grid_dep_launch();
   grid_dep_wait();
-  const int r = threadIdx.x, t = blockIdx.x & 1, col = blockIdx.y * 8;
+  const int r = threadIdx.x, t = blockIdx.x & 1, col = blockIdx.y * 4;
   const int item = blockIdx.x >> 1, idx = div_by(item, a.by_groups), group = item - idx * a.groups;
   const int in_tile = div_by(r, a.by_pack), tok = (2 * (a.pairs - 1 - idx) + t) * a.tpt + in_tile;
   const int head = group * a.pack + (r - in_tile * a.pack);
   const int rows = a.cu_q != nullptr ? a.total_q : a.B * a.Nq;
   if (in_tile >= a.tpt || tok >= rows) return;
   if (a.cu_q != nullptr && (tok < a.cu_q[0] || tok >= a.cu_q[a.B])) return;  // no sequence's
-  auto slot_row = [&](int p) { return ((static_cast<long long>(item) * n_parts + p) * 2 + t) * kTileM + r; };
   const long long rest = static_cast<long long>(tok) * a.Hq + head;
   const float2 ml_rest = a.rest_ml[rest];
-  float m = ml_rest.x;
-#pragma unroll 8
-  for (int p = 0; p < n_parts; ++p) m = fmaxf(m, a.part_ml[slot_row(p)].x);
-  float l = 0.f, o[8] = {};
-  auto add = [&](float2 ml, float4 y0, float4 y1) {
-    const float w = part_weight(ml.x, m);
-    l = fmaf(ml.y, w, l);
-    o[0] = fmaf(y0.x, w, o[0]);
-    o[1] = fmaf(y0.y, w, o[1]);
-    o[2] = fmaf(y0.z, w, o[2]);
-    o[3] = fmaf(y0.w, w, o[3]);
-    o[4] = fmaf(y1.x, w, o[4]);
-    o[5] = fmaf(y1.y, w, o[5]);
-    o[6] = fmaf(y1.z, w, o[6]);
-    o[7] = fmaf(y1.w, w, o[7]);
-  };
-  const float4* pr = reinterpret_cast<const float4*>(a.rest_o + rest * D + col);
-  add(ml_rest, pr[0], pr[1]);
-  constexpr int kAhead = 6;  // pieces whose loads are in flight together
+  const float4 y_rest = *reinterpret_cast<const float4*>(a.rest_o + rest * D + col);
+  float m = ml_rest.x, l = ml_rest.y, o[4] = {y_rest.x, y_rest.y, y_rest.z, y_rest.w};
+  if (m == -INFINITY) l = o[0] = o[1] = o[2] = o[3] = 0.f;
+  constexpr int kAhead = 16;  // pieces whose loads are in flight together
   for (int p0 = 0; p0 < n_parts; p0 += kAhead) {
-    float4 y[kAhead][2];
+    float4 y[kAhead];
     float2 ml[kAhead];
+    float top = m;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const long long at = slot_row(min(p0 + u, n_parts - 1));
-      const float4* po = reinterpret_cast<const float4*>(a.part_o + (at - r) * D) + (col / 4) * kTileM + r;
+      if (p0 + u >= n_parts) break;
+      const long long at = ((static_cast<long long>(item) * n_parts + p0 + u) * 2 + t) * kTileM + r;
       ml[u] = a.part_ml[at];
-      y[u][0] = po[0];
-      y[u][1] = po[kTileM];
+      y[u] = *(reinterpret_cast<const float4*>(a.part_o + (at - r) * D) + (col / 4) * kTileM + r);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (p0 + u < n_parts) add(ml[u], y[u][0], y[u][1]);
+      if (p0 + u < n_parts) top = fmaxf(top, ml[u].x);
+    const float keep = part_weight(m, top);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= keep;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (p0 + u < n_parts) {
+        const float w = part_weight(ml[u].x, m);
+        l = fmaf(ml[u].y, w, l);
+        o[0] = fmaf(y[u].x, w, o[0]);
+        o[1] = fmaf(y[u].y, w, o[1]);
+        o[2] = fmaf(y[u].z, w, o[2]);
+        o[3] = fmaf(y[u].w, w, o[3]);
+      }
   }
   const float f = l > 0.f ? 1.f / l : l;  // a NaN stays one
   long long seq = 0, at = tok;
@@ -822,9 +822,8 @@ cache_merge_kernel(const CacheArgs a, int n_parts) {
     seq = div_by(tok, a.by_nq);
     at = tok - seq * a.Nq;
   }
-  *reinterpret_cast<uint4*>(a.o + seq * a.os[0] + head * a.os[1] + at * a.os[2] + col) =
-      make_uint4(pack2<BF16>(o[0] * f, o[1] * f), pack2<BF16>(o[2] * f, o[3] * f), pack2<BF16>(o[4] * f, o[5] * f),
-                 pack2<BF16>(o[6] * f, o[7] * f));
+  *reinterpret_cast<uint2*>(a.o + seq * a.os[0] + head * a.os[1] + at * a.os[2] + col) =
+      make_uint2(pack2<BF16>(o[0] * f, o[1] * f), pack2<BF16>(o[2] * f, o[3] * f));
   if (col == 0 && a.lse != nullptr) a.lse[seq * a.ls[0] + head * a.ls[1] + at] = row_lse(m, l);
 }
 
@@ -862,7 +861,7 @@ cudaError_t launch_fwd_cache_ws(int D, bool bf16, bool prefix, const CUtensorMap
 
 // After launch_fwd_cache_ws over the prefix (`items` x `parts` pieces) and launch_fwd_cache over the rest.
 cudaError_t launch_cache_merge(int D, bool bf16, const CacheArgs& a, int items, int parts, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(items) * 2, a.D / 8);
+  const dim3 grid(static_cast<unsigned>(items) * 2, a.D / 4);
   if (D == 128)
     return bf16 ? launch_overlapped(cache_merge_kernel<128, true>, grid, 128, 0, st, a, parts)
                 : launch_overlapped(cache_merge_kernel<128, false>, grid, 128, 0, st, a, parts);
