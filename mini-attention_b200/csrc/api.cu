@@ -1049,11 +1049,11 @@ constexpr int kMinPieceTiles = 4;      // 128-key tiles of a piece
 constexpr int kMinPrefixTiles = 2;     // of a shared prefix's, whose pieces a launch of its own adds up
 constexpr long long kMaxPieces = 480;  // of all items together: 64 MB of scratch at D = 128
 
-// Pieces that items of at most `tiles` tiles are cut into where all are alike.  A CTA takes its tiles and about 4 steps of a tile's time beside
-// them; a piece takes 2 more to leave its result, the last 0.8 for each piece it folds.
-int cache_pieces(long long items, int tiles, int sms) {
+// Pieces that items of at most `tiles` tiles are cut into where all are alike.  A CTA takes its tiles and about 4 steps of a
+// tile's time beside them; a piece takes 2 more to leave its result, the last 0.8 for each piece it folds.
+int cache_pieces(long long items, int tiles, int sms, float* least_cost) {
   int best = 1;
-  float least = 0.f;
+  float& least = *least_cost;
   for (int n = 1; n <= 32 && (n == 1 || (n * items <= kMaxPieces && tiles / n >= kMinPieceTiles)); ++n) {
     const float rounds = static_cast<float>((items * n + sms - 1) / sms);
     const float cost = rounds * (static_cast<float>((tiles + n - 1) / n) + 4.f + (n > 1 ? 2.f + 0.8f * n : 0.f));
@@ -1111,13 +1111,21 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
     }
     return c;
   }
-  const long long seen = p->window > 0 ? std::min(room, static_cast<long long>(p->window) + p->sinks + span + 256) : room;
-  if (items <= kMaxPieces) c.parts = cache_pieces(items, tiles_of(seen), sms);
+  const auto seen_by = [&](long long tokens) {  // in tiles, at most
+    return tiles_of(p->window > 0 ? std::min(room, static_cast<long long>(p->window) + p->sinks + tokens + 256) : room);
+  };
+  float least = 0.f;
+  if (items <= kMaxPieces) c.parts = cache_pieces(items, seen_by(span), sms, &least);
+  // Few pairs are quicker taken apart, a Q tile to a CTA, than cut along the keys, unless their keys are many: a step of a single
+  // tile takes 0.8 of a pair's, and nothing is folded.  Apart / cut, D = 128: 2048 tokens of 8 heads, window 500 13.4 / 18.2 us,
+  // window 1000 17.4 / 22.3; a chunk of 128 tokens against 1024 keys, 32/8 heads 13.4 / 19.0, 512 against 2048, 8/2 heads 21.1 /
+  // 22.4 (D = 64 19.7 / 17.8), 2 x 200 against 8000 67.9 / 33.2.
+  if (c.parts > 1 && 2 * items <= sms && n > c.tpt && 0.8f * static_cast<float>(seen_by(c.tpt)) + 4.f < least) c.parts = 1;
   if (c.parts > 1) c.part_rows = static_cast<size_t>(items) * c.parts * 2 * ma::kTileM;
-  // A last wave that is at most half full: its pairs are taken apart, so that it ends sooner (not where a sequence has an odd
-  // number of Q tiles: half of the CTAs would have nothing to do).
+  // A last wave that is at most half full, or all of a call that fills no more: its pairs are taken apart, so that it ends
+  // sooner (12 heads of 128, 1024 tokens, window 256: 10.9 us, 14.7 in pairs).  Not where a sequence has one Q tile.
   const long long rest = items % sms;
-  if (c.parts == 1 && items > sms && rest > 0 && 2 * rest <= sms && (n + c.tpt - 1) / c.tpt % 2 == 0 && items < 0x3fffffff) {
+  if (c.parts == 1 && rest > 0 && 2 * rest <= sms && n > c.tpt && items < 0x3fffffff) {
     c.pair_items = static_cast<int>(items - rest);
     c.ctas = static_cast<int>(items + rest);
   }
