@@ -133,9 +133,11 @@ __device__ __forceinline__ void wait_for_copies() {
 // Which piece of which item CTA x of a ragged launch works on; the whole warp.  False: none.  Lengths are known here only, so
 // every CTA adds up the tiles of all sequences: pieces are at most half as long as an SM's share, and where the sequences are
 // few those with the most keys come first.  (One piece per pair, sequences in their order: 148 SMs wait for the last of 192
-// items of 100 tiles, 357 us where all items together are 237 on each SM.)
-__device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* it, int* pair) {
-  const int lane = threadIdx.x & 31, span = 2 * a.tpt;
+// items of 100 tiles, 357 us where all items together are 237 on each SM.)  Where single Q tiles fill no more than a CTA per SM
+// and no piece of a pair would be much shorter than they are, each is an item (*single: which of its pair).
+__device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* it, int* pair, int* single) {
+  const int lane = threadIdx.x & 31;
+  int span = 2 * a.tpt;
   auto look = [&](int b, CacheSeq* s, int* pairs, int* tiles) {
     *pairs = 0;
     *tiles = 1;
@@ -149,21 +151,34 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
   CacheSeq s{};
   int pairs, tiles, most = 0x7fffffff;  // tiles of a piece
   if (a.cut > 0) {
-    long long total = 0, items = 0;
+    long long total = 0, items = 0, apart = 0;
+    int longest = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       look(b0 + lane, &s, &pairs, &tiles);
       total += static_cast<long long>(pairs) * tiles;
       items += pairs;
+      if (pairs > 0) {
+        apart += (s.nq + (a.tpt - 1)) / a.tpt;
+        longest = max(longest, tiles);
+      }
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
       total += __shfl_xor_sync(0xffffffffu, total, d);
       items += __shfl_xor_sync(0xffffffffu, items, d);
+      apart += __shfl_xor_sync(0xffffffffu, apart, d);
     }
+    longest = __reduce_max_sync(0xffffffffu, longest);
     const long long even = (total * a.groups + a.cut - 1) / a.cut;
     // Rows that overlap, which only row numbers that fall give, may be more than the launch has CTAs for: a piece without one
     // would leave its item's counter standing, so nothing is cut then.
     if (items * a.groups + a.cut <= gridDim.x) most = clamp_to(even, 2 * a.min_tiles, 0x7fffffff);
+    // 2 x 128 tokens against 1600 keys, 32/8 heads of 128: 21.6 us, 26.2 in pieces of pairs; 300 against 2040, 8/2 heads 24.0
+    // and 27.0.  Not where most pairs are single tiles as it is (3 x 100 tokens, 12 heads: 24.9, 23.1 in pieces).
+    if (2 * apart * a.groups <= a.cut && 2 * apart >= 3 * items && longest <= max(most, 4 * a.min_tiles)) {
+      span = a.tpt;
+      most = 0x7fffffff;
+    }
   }
   long long before = 0;  // pieces of the sequences before
   for (int b0 = 0; b0 < a.B; b0 += 32) {
@@ -188,6 +203,10 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
       const int back = div_by(idx, a.by_groups);
       it->group = idx - back * a.groups;
       *pair = __shfl_sync(0xffffffffu, pairs, l) - 1 - back;  // the latest first: it sees the most keys
+      if (span == a.tpt) {
+        *single = *pair & 1;
+        *pair >>= 1;
+      }
       it->s = cache_seq(a, a.cu_q[it->b], a.cu_q[it->b + 1], a.seq_lens[it->b]);
       return true;
     }
@@ -279,7 +298,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         it.s = cache_seq(a, 0, 0, a.seq_lens != nullptr ? a.seq_lens[it.b] : 0);
       }
     } else {
-      there = ragged_item(a, x, &it, &pair);
+      there = ragged_item(a, x, &it, &pair, &single);
       it.slot0 = x - it.part;
     }
     if (there) {

@@ -184,6 +184,19 @@ def test_result_in_place_of_the_queries(lens, n, G, shared):
         check(q[b], o, t, f"sequence {b}")
 
 
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("lens,n,Hkv,G,D,window", [
+    ([1300, 900], 128, 2, 4, 128, None),    # Q tiles one by one
+    ([1100], 513, 4, 1, 64, None),          # an odd number of them
+    ([700, 2, 300], 150, 1, 3, 96, 40),     # the front of a sequence missing
+    ([3000, 2500], 100, 2, 4, 128, None),   # pairs, cut along the keys
+    ([640] * 10, 130, 2, 8, 64, 100),       # pairs
+    ([500] * 9, 260, 7, 1, 128, 300)])      # pairs, the last wave's one by one
+def test_chunks(lens, n, Hkv, G, D, window, ragged):
+    p = Paged(lens, [n] * len(lens), Hkv, D, BF16, 32, window=window, sinks=3 if window else 0, seed=41)
+    _compare(p, _queries(p.news, Hkv * G, D, BF16), ragged)
+
+
 @pytest.mark.parametrize("n,G,D", [(1, 129, 64), (3, 129, 128), (20, 129, 128), (2, 200, 96)])
 def test_more_heads_than_a_tile_has_rows(n, G, D):
     p = Paged([700, 41, 5], [n, n, n], 1, D, F16, 16, seed=32)
