@@ -1084,8 +1084,9 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
     const bool stacked = ragged || (p->Nq == 1 ? p->q_stride[0] >= p->D || p->B == 1 : p->q_stride[0] == p->Nq * p->q_stride[2]);
     const long long all = ragged ? p->total_q : static_cast<long long>(p->B) * p->Nq, pairs = (all + span - 1) / span;
     // What all sequences would read of it without: the two launches more and the pieces between them cost about as much as
-    // 100 MB of it.  With and without, 32/8 heads of 128: 16 x 1024 tokens (67 MB) 21.5 / 17.5 us, 64 x 512 (134) 29.0 / 28.8,
-    // 16 x 4096 (268) 23.8 / 36.1, 64 x 2048 (537) 31.1 / 67.7; 64 x 2048, 8/2 heads of 64 (67) 16.9 / 18.8.
+    // 100 MB of it.  With and without, 32/8 heads of 128: 16 x 1024 tokens (67 MB) 17.1 / 15.9 us, 64 x 512 (134) 27.1 / 26.1,
+    // 32 x 1024 (134) 18.2 / 22.2, 16 x 4096 (268) 18.9 / 29.5, 64 x 2048 (537) 29.7 / 53.7; 8/2 heads of 64: 64 x 2048 (67)
+    // 16.8 / 16.8.
     const long long row_blocks = (rows + 16 * c.rg - 1) / (16 * c.rg);
     const double read = 4.0 * p->B * p->Hkv * row_blocks * p->shared_len * kernel_head_dim(p->D);
     if (read >= 1e8 && p->n_pages > 0 && stacked && pairs * c.groups <= kMaxPieces) {

@@ -18,13 +18,18 @@
 // 1.7 us a 128-key step of a CTA at the power cap).  Short windows are bound by a CTA's ends and by the tiles that only some of
 // its 256 rows see: 4 x 1024 tokens, 12 heads of 64, window 256 20.6 us, 3 us of an item's 12 outside its steps.
 //
+// Few items: their pairs are taken apart, a Q tile to a CTA; a CTA's step then takes 0.8 of a pair's and there is nothing to
+// fold (rules and figures: cache_plan in api.cu, ragged_item).
+//
 // The query heads of a KV head always share Q tiles: a pair of tiles then spans 256 / G tokens, and its band of keys is that
 // much narrower.
 //
 // Built and dropped: one CTA an SM that walks a contiguous part of all items' tiles (cut evenly, no second wave).  Its start
 // takes 4.5 us instead of 1.5, and without the offset that each item gives its second Q tile the two softmax groups fall into
 // step, in which a 64-key half takes 1750 clk instead of 1520: both calls above took 14 % longer, only mixed chunks gained.  Turns
-// that keep the groups apart, through a barrier between the MMA warps, cost more than the step (2000 clk).
+// that keep the groups apart, through a barrier between the MMA warps, cost more than the step (2000 clk).  Two CTAs of one Q tile
+// each on an SM (D = 64, four ring slots, half of TMEM): as quick as single tiles on SMs of their own where those fit, and 4096
+// tokens, 12 heads, window 1024 took 106 us instead of 98.7, 1024 tokens, window 256 the same: the groups fall into step.
 #include <atomic>
 
 #include "cache.cuh"
