@@ -335,6 +335,31 @@ def test_captured_call_serves_longer_contexts():
     miniattn.check_device_status(DEV)
 
 
+@pytest.mark.parametrize("lens,n,G,shared", [([3000, 1700], 1, 4, 0), ([3000, 2900], 40, 4, 0),
+                                             ([1100 + 17 * i for i in range(48)], 1, 8, 1024)])
+def test_two_graphs_at_once(lens, n, G, shared):
+    """Captured calls share no scratch: replayed on two streams, with an eager call beside them, they give what they give alone."""
+    p = Paged(lens, [n] * len(lens), 4, 128, BF16, 32, seed=9, shared=shared)
+    q = torch.stack(_queries(p.news, 4 * G, 128, BF16)).to(DEV)
+    call = lambda: miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, shared_len=shared)
+    want = call()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = [call() for _ in range(4)]
+        graphs.append((g, out, torch.cuda.Stream()))
+    for _ in range(5):
+        for g, _, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = [call() for _ in range(4)]
+    torch.cuda.synchronize()
+    for out in (graphs[0][1], graphs[1][1], eager):
+        assert all(torch.equal(o, want) for o in out)
+
+
 def test_captured_ragged_call_serves_other_batches():
     """One graph of a ragged call, replayed for batches of other rows and lengths (its grid knows the sizes of q alone)."""
     from paged_reference import attention
