@@ -45,9 +45,12 @@ def _serve(projected, w_o, n_kv_heads, head_dim, k_cache, v_cache, block_table, 
     rows = q.shape[:-1]
     q = q.view(*rows, -1, head_dim)
     kv = kv.view(*rows, 2, n_kv_heads, head_dim)
-    turned = q if rope is not None else None   # in place: nobody else has seen it
-    paged_append(kv[..., 0, :, :], kv[..., 1, :, :], k_cache, v_cache, block_table, seq_lens, cu_q=cu_q, q=turned, q_out=turned,
-                 rope=rope, interleaved=interleaved)
+    new = (kv[..., 0, :, :], kv[..., 1, :, :], k_cache, v_cache, block_table, seq_lens)
+    if rope is None:
+        paged_append(*new, cu_q=cu_q)
+    else:
+        # In place only in the one launch's own output: what a layer's call returned, a hook or the caller may hold as well.
+        q = paged_append(*new, cu_q=cu_q, q=q, q_out=q if type(projected) is tuple else None, rope=rope, interleaved=interleaved)
     o = paged_attention(q, k_cache, v_cache, block_table, seq_lens, cu_q=cu_q, max_q=max_q, window=window, sinks=sinks,
                         shared_len=shared_len)
     return _project(o.reshape(*rows, -1), w_o, projected)
