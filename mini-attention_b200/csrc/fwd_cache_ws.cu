@@ -808,7 +808,9 @@ cache_merge_kernel(const CacheArgs a, int n_parts) {
   const float2 ml_rest = a.rest_ml[rest];
   const float4 y_rest = *reinterpret_cast<const float4*>(a.rest_o + rest * D + col);
   float m = ml_rest.x, l = ml_rest.y, o[4] = {y_rest.x, y_rest.y, y_rest.z, y_rest.w};
-  if (m == -INFINITY) l = o[0] = o[1] = o[2] = o[3] = 0.f;
+  // A row without keys in the rest: its sum is 0.  A row maximum of -inf does not say so: that of the launch over the rest
+  // passes over NaN, and a row all of whose keys score one has it beside a sum that is NaN.
+  if (l == 0.f) o[0] = o[1] = o[2] = o[3] = 0.f;
   constexpr int kAhead = 16;  // pieces whose loads are in flight together
   for (int p0 = 0; p0 < n_parts; p0 += kAhead) {
     float4 y[kAhead];

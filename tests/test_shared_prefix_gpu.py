@@ -1,0 +1,54 @@
+"""miniattn.paged_attention behind a shared prefix that a launch of its own reads: what one sequence holds that is not a number,
+out of range or nobody's stays its own."""
+import pytest
+import torch
+
+import miniattn
+from paged_reference import Paged, check
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16 = torch.bfloat16
+SHARED, HKV, HQ, D, PAGE, B = 1024, 8, 32, 128, 32, 48   # 200 MB would be read without: a launch of its own
+OUTSIDE = 10 ** 6                                          # no page of the cache
+
+
+def _batch(lens, news, seed):
+    p = Paged(lens, news, HKV, D, BF16, PAGE, shared=SHARED, seed=seed)
+    gen = torch.Generator().manual_seed(seed + 1)
+    return p, [torch.randn((n, HQ, D), generator=gen).to(BF16) for n in news]
+
+
+def _call(p, rows, ragged, shared=SHARED):
+    """Output (n,Hq,D) and lse (Hq,n) of each sequence."""
+    if ragged:
+        out, lse = miniattn.paged_attention(torch.cat(rows).to(DEV), p.k_cache, p.v_cache, p.table, p.seq_lens, cu_q=p.cu_q,
+                                            max_q=max(p.news), shared_len=shared, return_lse=True)
+        return list(out.split(p.news)), list(lse.split(p.news, 1))
+    out, lse = miniattn.paged_attention(torch.stack(rows).to(DEV), p.k_cache, p.v_cache, p.table, p.seq_lens,
+                                        shared_len=shared, return_lse=True)
+    return list(out), list(lse)
+
+
+def _right(p, rows, outs, lses, but=()):
+    for b, (o, t, z, tz) in enumerate(zip(*p.expected(rows))):
+        if b not in but:
+            check(outs[b], o, t, f"sequence {b}")
+            check(lses[b], z, tz, f"lse of sequence {b}")
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_a_row_whose_own_keys_are_nan(ragged):
+    """The first token after the prefix is the only key that the launch over the rest sees of sequence 5: a NaN there is one in the
+    row's result, for the query heads of that KV head, as it is without the prefix."""
+    p, rows = _batch([SHARED + 1] * B, [1] * B, seed=51)
+    p.k_cache[int(p.table[5, SHARED // PAGE]), 0, 3] = float("nan")
+    for shared in (0, SHARED):
+        outs, lses = _call(p, rows, ragged, shared)
+        heads = torch.zeros(HQ, dtype=torch.bool, device=DEV)
+        heads[12:16] = True
+        assert torch.equal(outs[5][0].isnan(), heads[:, None].expand(HQ, D)) and torch.equal(lses[5][:, 0].isnan(), heads)
+        _right(p, rows, outs, lses, but=(5,))
+    o, t, z, tz = (x[5] for x in p.expected(rows))
+    check(outs[5][:, ~heads], o[:, ~heads], t[:, ~heads], "the other heads")
+    miniattn.check_device_status(DEV)
