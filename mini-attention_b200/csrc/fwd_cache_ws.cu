@@ -833,7 +833,9 @@ cache_merge_kernel(const CacheArgs a, int n_parts) {
     for (int i = 0; i < 4; ++i) o[i] *= keep;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (p0 + u < n_parts) {
+      // A piece of which the row sees no key is left out, not weighted with 0: its O is 0 times the values that other sequences
+      // see, which an infinity or a NaN among them makes a NaN.
+      if (p0 + u < n_parts && ml[u].y != 0.f) {
         const float w = part_weight(ml[u].x, m);
         l = fmaf(ml[u].y, w, l);
         o[0] = fmaf(y[u].x, w, o[0]);

@@ -52,3 +52,16 @@ def test_a_row_whose_own_keys_are_nan(ragged):
     o, t, z, tz = (x[5] for x in p.expected(rows))
     check(outs[5][:, ~heads], o[:, ~heads], t[:, ~heads], "the other heads")
     miniattn.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_values_of_the_prefix_that_are_no_numbers(value):
+    """They are in the results of all who see them; a sequence of length 0 sees nothing, its rows are 0."""
+    lens = [0] + [SHARED + 1 + i for i in range(B - 1)]
+    p, rows = _batch(lens, [1] * B, seed=52)
+    p.v_cache[int(p.table[1, 7]), 9, 2, 17] = value
+    outs, lses = _call(p, rows, False)
+    assert bool((outs[0] == 0).all()) and bool((lses[0] == -float("inf")).all())
+    for b in range(1, B):
+        odd = ~outs[b][0].isfinite()
+        assert bool(odd[8:12, 17].all()) and int(odd.sum()) == 4
