@@ -290,13 +290,19 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       it.slot0 = x * static_cast<int>(gridDim.y);
       if constexpr (PREFIX) {
         it.s.nq = a.cu_q != nullptr ? a.total_q : a.B * a.Nq;
-        // read through the block table of the longest sequence: others may be padding, or end before the prefix does
+        // Read through the block table of the longest sequence: others may be padding, or end before the prefix does.  Only a
+        // sequence that has rows and whose rows and length are in range: nobody needs the pages of the others.
+        const auto usable = [&](int b) {
+          const CacheSeq s = cache_seq(a, a.cu_q != nullptr ? a.cu_q[b] : 0, a.cu_q != nullptr ? a.cu_q[b + 1] : 0, a.seq_lens[b]);
+          return s.nq > 0 && !s.bad;
+        };
         int longest = -1;
-        for (int b = lane; b < a.B; b += 32) longest = max(longest, a.seq_lens[b]);
-        longest = __reduce_max_sync(0xffffffffu, longest);
-        int of = 0x7fffffff;
         for (int b = lane; b < a.B; b += 32)
-          if (a.seq_lens[b] == longest) of = min(of, b);
+          if (usable(b)) longest = max(longest, a.seq_lens[b]);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        int of = a.B - 1;
+        for (int b = lane; b < a.B; b += 32)
+          if (a.seq_lens[b] == longest && usable(b)) of = min(of, b);
         it.b = __reduce_min_sync(0xffffffffu, of);
         it.s.hi = clamp_to(min(a.shared, longest), 0, static_cast<long long>(a.table_width) << a.page_shift);
       } else {

@@ -65,3 +65,40 @@ def test_values_of_the_prefix_that_are_no_numbers(value):
     for b in range(1, B):
         odd = ~outs[b][0].isfinite()
         assert bool(odd[8:12, 17].all()) and int(odd.sum()) == 4
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("length", [10 ** 9, -3])
+def test_a_length_that_is_out_of_range(length, ragged):
+    """Reported; the others are right, although the spoiled slot's row of the block table holds no pages."""
+    lens = [SHARED + 5 + 11 * i for i in range(B)]
+    p, rows = _batch(lens, [1] * B, seed=53)
+    p.seq_lens[1] = length
+    p.table[1] = OUTSIDE
+    outs, lses = _call(p, rows, ragged)
+    with pytest.raises(RuntimeError, match="outside its tensors"):
+        miniattn.check_device_status(DEV)
+    _right(p, rows, outs, lses, but=(1,))
+
+
+def test_a_sequence_without_rows():
+    """Nobody needs its tokens: its length may be an old one, its pages somebody else's by now."""
+    news = [1] * B
+    news[4] = 0
+    lens = [SHARED + 5 + 11 * i for i in range(B)]
+    lens[4] = SHARED + 900   # the longest
+    p, rows = _batch(lens, news, seed=54)
+    p.table[4] = OUTSIDE
+    outs, lses = _call(p, rows, True)
+    _right(p, rows, outs, lses)
+    miniattn.check_device_status(DEV)
+
+
+def test_no_length_in_range():
+    """Nothing is read; reported."""
+    p, rows = _batch([SHARED + 1] * B, [1] * B, seed=55)
+    p.seq_lens.fill_(-1)
+    p.table.fill_(OUTSIDE)
+    _call(p, rows, False)
+    with pytest.raises(RuntimeError, match="outside its tensors"):
+        miniattn.check_device_status(DEV)
