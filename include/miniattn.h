@@ -351,7 +351,9 @@ typedef struct MiniAttnCacheParams {
   float   softmax_scale;  /* <= 0 selects 1/sqrt(D)                                    */
 } MiniAttnCacheParams;
 
-/* scratch: as for miniattn_fwd_balanced, miniattn_fwd_cache_scratch_bytes(p) bytes; not optional.  That size depends on the
+/* scratch: as for miniattn_fwd_balanced, miniattn_fwd_cache_scratch_bytes(p) bytes; not optional.  With shared_len
+ * the call may make several launches that hand results on in it: between them no other thread may enqueue a call that uses the same
+ * scratch, so threads that share a stream need a scratch each, or a lock around the call.  That size depends on the
  * sizes in `p` alone; pointers are compared with null and not read. */
 int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scratch_bytes, void* stream);
 int64_t miniattn_fwd_cache_scratch_bytes(const MiniAttnCacheParams* p);

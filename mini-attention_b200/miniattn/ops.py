@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import threading
 from typing import Optional, Tuple, Union
 
 import torch
@@ -22,6 +23,7 @@ _status_words: dict = {}
 _COUNTER_BYTES = 16384        # arrival counters at the start of a balanced launch's scratch
 _balance_scratch: dict = {}   # (device index, stream) -> zero-initialised uint8 scratch tensor
 _capture_scratch: dict = {}   # the same for the last capture on that stream: (capture id, scratch of the graph)
+_together_locks: dict = {}    # (device index, stream) -> what a call of several launches holds while it makes them
 # Parameter blocks of recent calls, keyed by everything that goes into one (pointers, shapes, strides,
 # dtype, flags).  A training or serving loop calls the operator with the same tensors again and again;
 # validating and filling the block costs more host time than a short-sequence kernel runs for.
@@ -66,12 +68,13 @@ def check_device_status(device: Union[torch.device, str, None] = None) -> None:
                "device status")
 
 
-def _scratch_for(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+def _scratch_for(device: torch.device, stream: int, nbytes: int, *together) -> torch.Tensor:
     """Scratch of a balanced launch: one buffer per (device, stream), zeroed when created (the
     kernels leave the arrival counters at its start zero again), grown on demand.  A call that is being
     captured gets one of the graph's own memory, since the graph may be replayed on any stream: one buffer
-    for all calls that one capture makes on a stream, its counters cleared by the graph before the first."""
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+    for all calls that one capture makes on a stream, its counters cleared by the graph before the first.
+    `together` tells buffers of one stream apart (:func:`_launch_together`)."""
+    key = (device.index if device.index is not None else torch.cuda.current_device(), stream, *together)
     if torch.cuda.is_current_stream_capturing():
         capture = C.c_uint64(0)
         _lib.check(_lib.lib.miniattn_stream_capture_id(stream, C.byref(capture)), "miniattn_stream_capture_id")
@@ -352,7 +355,7 @@ def _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q
     device = q.device
     status = _status_words.get(("cuda", device.index))
     _launch_cache(_pack_cache(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                              (_status_word(device) if status is None else status).data_ptr(), 0, 0, 0) + rest, need, device)
+                              (_status_word(device) if status is None else status).data_ptr(), 0, 0, 0) + rest, need, device, False)
     return (out, lse) if return_lse else out
 
 
@@ -364,20 +367,34 @@ def _cache_scratch_bytes(p, device: torch.device) -> int:
     return need
 
 
-def _launch_cache(block: bytes, need: int, device: torch.device) -> None:
-    """``miniattn_fwd_cache`` of a packed parameter block on the current stream of `device`, with the scratch of that stream."""
+def _launch_cache(block: bytes, need: int, device: torch.device, several: bool) -> None:
+    """``miniattn_fwd_cache`` of a packed parameter block on the current stream of `device`, with the scratch of that stream.
+    `several`: it may take more than one launch."""
+    launch = _launch_together if several else _launch_cache_on
     if _current_device() == device.index:
-        rc = _launch_cache_on(block, need, device, _current_raw_stream(device.index))
+        rc = launch(block, need, device, _current_raw_stream(device.index))
     else:
         with torch.cuda.device(device.index):
-            rc = _launch_cache_on(block, need, device, _current_raw_stream(device.index))
+            rc = launch(block, need, device, _current_raw_stream(device.index))
     if rc != _lib.OK:
         _lib.check(rc, "miniattn_fwd_cache")
 
 
-def _launch_cache_on(block: bytes, need: int, device: torch.device, stream: int) -> int:
-    scratch = _scratch_for(device, stream, need)
+def _launch_cache_on(block: bytes, need: int, device: torch.device, stream: int, *together) -> int:
+    scratch = _scratch_for(device, stream, need, *together)
     return _lib.lib.miniattn_fwd_cache(block, scratch.data_ptr(), scratch.numel(), stream)
+
+
+def _launch_together(block: bytes, need: int, device: torch.device, stream: int) -> int:
+    """A call of several launches, which hand results on in scratch.  ctypes lets other host threads run during a call, and threads
+    share torch's default stream: launches of theirs that come between must not use the same scratch.  So such calls take turns on
+    a stream, and have a scratch there that no other call uses."""
+    key = (device.index, stream)
+    lock = _together_locks.get(key)
+    if lock is None:
+        lock = _together_locks.setdefault(key, threading.RLock())
+    with lock:
+        return _launch_cache_on(block, need, device, stream, "together")
 
 
 # cudaStream_t of torch's current stream on a device without building a Stream object, and the current device

@@ -298,5 +298,5 @@ def paged_attention(
         _launch_cache(_pack_attend(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
             (_status_word(device) if status is None else status).data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-            0 if cu_q is None else cu_q.data_ptr()) + rest, need, device)
+            0 if cu_q is None else cu_q.data_ptr()) + rest, need, device, shared_len > 0)
     return (out, lse) if return_lse else out
