@@ -10,6 +10,7 @@ device memory and streams only; the arithmetic runs in libminiattn.so.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import struct
 import threading
 from typing import Optional, Tuple, Union
@@ -313,8 +314,33 @@ _window_forms: dict = {}   # what follows from the form of a call with a window,
 _pack_cache = struct.Struct("@9P").pack   # the pointers of MiniAttnCacheParams
 
 
+def _as_int(name: str, x) -> int:
+    """A whole number of a call as an int.  What is kept of a call goes by its numbers: a tensor is found again by its identity,
+    whatever it holds by then."""
+    if isinstance(x, torch.Tensor):
+        x = x.item()
+    try:
+        return operator.index(x)
+    except TypeError:
+        pass
+    if isinstance(x, float) and x.is_integer():
+        return int(x)
+    raise RuntimeError(f"{name} must be a whole number, got {x!r}")
+
+
 def _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q_pos0, k_pos0, window, sinks):
     """``flash_attn_fwd`` with a sliding window."""
+    if window is not None and type(window) is not int:
+        window = _as_int("window", window)
+    if type(sinks) is not int:
+        sinks = _as_int("sinks", sinks)
+    if type(q_pos0) is not int:
+        q_pos0 = _as_int("q_pos0", q_pos0)
+    if type(k_pos0) is not int:
+        k_pos0 = _as_int("k_pos0", k_pos0)
+    if softmax_scale is not None and type(softmax_scale) is not float:
+        softmax_scale = float(softmax_scale)
+    causal = bool(causal)
     try:
         key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, q.get_device(),
                k.get_device(), v.get_device(), None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()),
@@ -341,7 +367,7 @@ def _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q
         p.lse_stride[:] = (f.Hq * f.Nq, f.Nq)
         p.diag = f.q_pos0 - f.k_pos0
         p.B, p.Hq, p.Hkv, p.D, p.Nq, p.Nk = f.B, f.Hq, f.Hkv, f.D, f.Nq, f.Nk
-        p.window, p.sinks = int(window), max(0, min(_INT32_MAX, int(sinks) - f.k_pos0))
+        p.window, p.sinks = window, max(0, min(_INT32_MAX, sinks - f.k_pos0))
         p.dtype, p.softmax_scale = f.dtype, f.softmax_scale
         form = (bytes(p)[9 * struct.calcsize("P"):], _cache_scratch_bytes(p, q.device), (f.B, f.Hq, f.Nq))
         if len(_window_forms) >= _PARAM_CACHE_MAX:

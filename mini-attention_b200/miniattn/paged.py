@@ -26,7 +26,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .ops import (_DTYPES, _INT32_MAX, _cache_scratch_bytes, _current_device, _current_raw_stream, _launch_cache, _status_word,
+from .ops import (_DTYPES, _INT32_MAX, _as_int, _cache_scratch_bytes, _current_device, _current_raw_stream, _launch_cache, _status_word,
                   _status_words)
 
 # What follows from the shapes, strides, dtypes and devices of a call, once they have been checked: the part of the parameter
@@ -79,10 +79,10 @@ def _check_ints(name: str, t, like: torch.Tensor, shape: Tuple[Optional[int], ..
         raise RuntimeError(f"{name} must be contiguous in its last dimension")
 
 
-def _whole(name: str, x, low: int) -> int:
+def _whole(name: str, x: int, low: int) -> int:
     if x < low or x > _INT32_MAX:
         raise RuntimeError(f"{name} must be between {low} and {_INT32_MAX}, got {x}")
-    return int(x)
+    return x
 
 
 def _check_paged(new: torch.Tensor, k_cache, v_cache, block_table, seq_lens, cu_q) -> int:
@@ -156,6 +156,7 @@ def paged_append(
 
     Returns the rotated queries, or None without ``q``.
     """
+    interleaved = bool(interleaved)
     try:
         key = (_form(k), _form(v), _form(k_cache), _form(v_cache), _form(block_table), _form(seq_lens), _form(cu_q), _form(q),
                _form(q_out), _form(rope), interleaved)
@@ -249,6 +250,16 @@ def paged_attention(
     Returns ``out`` or ``(out, lse)``, lse fp32, the natural logarithm of the softmax denominators: (B, Hq, n), or (Hq, rows)
     with ``cu_q``.  A NaN or infinity among the values of a key that any row of a sequence sees may show in others of its rows.
     """
+    if max_q is not None and type(max_q) is not int:
+        max_q = _as_int("max_q", max_q)
+    if window is not None and type(window) is not int:
+        window = _as_int("window", window)
+    if type(sinks) is not int:
+        sinks = _as_int("sinks", sinks)
+    if type(shared_len) is not int:
+        shared_len = _as_int("shared_len", shared_len)
+    if softmax_scale is not None and type(softmax_scale) is not float:
+        softmax_scale = float(softmax_scale)
     try:
         key = (_form(q), _form(k_cache), _form(v_cache), _form(block_table), _form(seq_lens), _form(cu_q), _form(out), max_q,
                window, sinks, shared_len, softmax_scale)
@@ -284,7 +295,7 @@ def paged_attention(
         p.window = _whole("window", window, 1) if window is not None else 0
         p.sinks, p.shared_len = _whole("sinks", sinks, 0), _whole("shared_len", shared_len, 0)
         p.dtype = _DTYPES[q.dtype]
-        p.softmax_scale = float(softmax_scale) if softmax_scale is not None else 0.0
+        p.softmax_scale = softmax_scale if softmax_scale is not None else 0.0
         need = _cache_scratch_bytes(p, q.device)
         lse_shape = (B, Hq, q.shape[1]) if cu_q is None else (Hq, q.shape[0])
         form = _keep(_attend_forms, key, (bytes(p)[_ATTEND_POINTERS:], need, lse_shape))
