@@ -234,6 +234,15 @@ def flash_attn_fwd(
         if carry is not None or carry_in or carry_out or carry_rows is not None:
             raise RuntimeError("a window and a carried state do not go together")
         return _windowed(q, k, v, causal, softmax_scale, layout, return_lse, out, kernel, q_pos0, k_pos0, window, sinks)
+    # as numbers: a tensor among them would be found again in the key below by its identity, whatever it holds by then
+    if type(q_pos0) is not int:
+        q_pos0 = int(q_pos0)
+    if type(k_pos0) is not int:
+        k_pos0 = int(k_pos0)
+    if softmax_scale is not None and type(softmax_scale) is not float:
+        softmax_scale = float(softmax_scale)
+    if carry_rows is not None:
+        carry_rows = tuple(int(x) for x in carry_rows)
     use_carry = bool(carry_in or carry_out)
     if use_carry and carry is None:
         raise RuntimeError("carry_in / carry_out need a carry buffer (carry_state)")
@@ -553,6 +562,7 @@ class HostPipeline:
     def _params(self, causal, softmax_scale, kernel):
         """Parameter blocks of the chunk launches: the staging tensors never move, so the blocks
         (and the scratch size of the balanced launch) are built once per (causal, scale, kernel)."""
+        softmax_scale = None if softmax_scale is None else float(softmax_scale)   # a tensor would be found again by its identity
         key = (bool(causal), softmax_scale, kernel)
         entry = self._launches.get(key)
         if entry is None:

@@ -40,6 +40,21 @@ def test_changed_in_place(call, name, values, rest):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name,values", [("softmax_scale", (0.5, 0.01)), ("q_pos0", (260, 100)), ("k_pos0", (0, 100))])
+def test_changed_in_place_without_a_window(name, values):
+    gen = torch.Generator().manual_seed(76)
+    q, k, v = (torch.randn((1, 2, n, 64), generator=gen).to(BF16).to(DEV) for n in (40, 300, 300))
+    out = torch.empty_like(q)
+    call = lambda x: miniattn.flash_attn_fwd(q, k, v, causal=True, out=out, **{"q_pos0": 260, name: x}).clone()  # noqa: E731
+    held = torch.tensor(values[0])
+    first = call(held)
+    assert torch.equal(first, call(values[0]))
+    held.fill_(values[1])
+    again = call(held)
+    assert torch.equal(again, call(values[1])) and not torch.equal(again, first)
+
+
+@pytest.mark.gpu
 def test_max_q():
     p = Paged([700, 90], [2, 60], 2, 64, BF16, 16, seed=74)
     q = torch.randn((62, 4, 64), generator=torch.Generator().manual_seed(75)).to(BF16).to(DEV)
