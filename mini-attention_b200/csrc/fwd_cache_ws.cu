@@ -155,6 +155,12 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
   };
   CacheSeq s{};
   int pairs, tiles, most = 0x7fffffff;  // tiles of a piece
+  // Sequences out of range are reported by the first CTA for all, since those left without rows are nobody's item.
+  if (x == 0 && a.status != nullptr) {
+    bool bad = false;
+    for (int b = lane; b < a.B; b += 32) bad |= cache_seq(a, a.cu_q[b], a.cu_q[b + 1], a.seq_lens[b]).bad;
+    if (bad) atomicOr(a.status, kErrCache);
+  }
   if (a.cut > 0) {
     long long total = 0, items = 0, apart = 0;
     int longest = 0;
