@@ -156,6 +156,11 @@ append_kernel(const AppendArgs a) {
       }
     }
   }
+  // A row reports what is wrong with its own sequence; sequences that no row finds by their numbers are looked at here, last, since
+  // the stores of the rows take longer to leave than this.
+  if (blockIdx.x == 0 && a.cu_q != nullptr && a.status != nullptr)
+    for (int b = threadIdx.x; b < a.B; b += kThreads)
+      if (append_outside(a, a.cu_q[b], a.cu_q[b + 1], a.seq_lens[b])) atomicOr(a.status, kErrCache);
 }
 
 template <bool BF16>

@@ -23,6 +23,12 @@ struct AppendArgs {
   FastDiv by_n, by_units;
 };
 
+// Whether a sequence of a ragged call lies outside its tensors, also one that no row of the call belongs to.
+__host__ __device__ inline bool append_outside(const AppendArgs& a, int first_row, int end_row, int seq_len) {
+  return first_row < 0 || end_row < first_row || end_row > a.rows || seq_len < 0 ||
+         seq_len > static_cast<long long>(a.table_width) << a.page_shift;
+}
+
 // Where row t of a sequence goes.
 struct AppendSlot {
   bool none;            // the row belongs to no sequence: it is left as it is, and so is its query

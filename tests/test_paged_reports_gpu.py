@@ -43,3 +43,29 @@ def test_chunks_in_order_are_not_reported():
     q = torch.zeros((400, 8, 64), dtype=BF16, device=DEV)
     miniattn.paged_attention(q, p.k_cache, p.v_cache, p.table, p.seq_lens, cu_q=p.cu_q)
     miniattn.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("total", [8, 3000])   # few rows and many: a CTA to a row, a warp to a row
+@pytest.mark.parametrize("cu,lens", [
+    ([5, 0, 4], [9, 30]),              # fall at once: no row is the first sequence's
+    ([0, 8, 4001, 4005], [9, 30, 9]),  # behind the rows: no row at all
+    ([-9, -4, 8], [9, 30]),            # in front of them
+    ([0, 1, 2, 3, 0], [9, 9, 9, 9]),
+    ([0, 8, 8], [9, -1]), ([0, 8, 8], [9, 10 ** 6])])
+def test_append(cu, lens, total):
+    B = len(lens)
+    caches = [torch.zeros((2 * B, 16, 2, 64), dtype=BF16, device=DEV) for _ in range(2)]
+    table = torch.arange(2 * B, dtype=torch.int32, device=DEV).view(B, 2)
+    k = torch.ones((total, 2, 64), dtype=BF16, device=DEV)
+    miniattn.paged_append(k, k, *caches, table, _ints(lens), cu_q=_ints(cu))
+    with pytest.raises(RuntimeError, match="outside its tensors"):
+        miniattn.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("total", [8, 3000])
+def test_append_in_order_is_not_reported(total):
+    caches = [torch.zeros((6, 16, 2, 64), dtype=BF16, device=DEV) for _ in range(2)]
+    table = torch.arange(6, dtype=torch.int32, device=DEV).view(3, 2)
+    k = torch.ones((total, 2, 64), dtype=BF16, device=DEV)
+    miniattn.paged_append(k, k, *caches, table, _ints([9, 32, 0]), cu_q=_ints([2, 6, 6, 8]))
+    miniattn.check_device_status(DEV)
