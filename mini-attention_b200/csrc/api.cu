@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <vector>
@@ -993,6 +994,12 @@ static int check_table(const int32_t* table, int64_t stride, int width, int page
   return MINIATTN_OK;
 }
 
+static int check_words(std::initializer_list<const void*> words) {
+  for (const void* w : words)
+    if (reinterpret_cast<uintptr_t>(w) % 4 != 0) return fail(MINIATTN_EINVAL, "cu_q, lse and status must be 4-byte aligned");
+  return MINIATTN_OK;
+}
+
 // Returns 1 when there is nothing to do.
 static int check_cache_sizes(const MiniAttnCacheParams* p) {
   if (p == nullptr) return fail(MINIATTN_EINVAL, "params is null");
@@ -1160,6 +1167,7 @@ int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scrat
   g_err[0] = 0;
   int rc = check_cache_sizes(p);
   if (rc != 0) return rc == 1 ? MINIATTN_OK : rc;
+  if ((rc = check_words({p->cu_q, p->lse, p->status})) != 0) return rc;
   if ((rc = check_tensor(p->q, p->q_stride, p->D, "q")) != 0 || (rc = check_tensor(p->o, p->o_stride, p->D, "o")) != 0) return rc;
   const bool paged = p->page_size != 0;
   const bool has_keys = paged ? p->n_pages > 0 && p->table_width > 0 : p->Nk > 0;
@@ -1294,6 +1302,7 @@ int miniattn_paged_append(const MiniAttnAppendParams* p, void* stream) {
   if (rows > 0x7fffffff) return fail(MINIATTN_EUNSUPPORTED, "the number of rows must fit in 31 bits");
   int rc;
   if ((rc = check_table(p->block_table, p->table_stride, p->table_width, p->page_size, p->n_pages, p->seq_lens)) != 0) return rc;
+  if ((rc = check_words({p->cu_q, p->status})) != 0) return rc;
   if (p->rope != nullptr) {
     if (p->rot < 16 || p->rot > p->D || p->rot % 16 != 0)
       return fail(MINIATTN_EUNSUPPORTED, "rot (%d) must be a multiple of 16 up to the head dim (%d)", p->rot, p->D);
