@@ -43,7 +43,7 @@ def _serve(projected, w_o, n_kv_heads, head_dim, k_cache, v_cache, block_table, 
     """The rest of ``forward_paged`` after the projections of q and of k and v."""
     q, kv = projected
     rows = q.shape[:-1]
-    q = q.view(*rows, -1, head_dim)
+    q = q.view(*rows, q.shape[-1] // head_dim, head_dim)   # counted, not -1: there may be no rows
     kv = kv.view(*rows, 2, n_kv_heads, head_dim)
     new = (kv[..., 0, :, :], kv[..., 1, :, :], k_cache, v_cache, block_table, seq_lens)
     if rope is None:
@@ -53,7 +53,7 @@ def _serve(projected, w_o, n_kv_heads, head_dim, k_cache, v_cache, block_table, 
         q = paged_append(*new, cu_q=cu_q, q=q, q_out=q if type(projected) is tuple else None, rope=rope, interleaved=interleaved)
     o = paged_attention(q, k_cache, v_cache, block_table, seq_lens, cu_q=cu_q, max_q=max_q, window=window, sinks=sinks,
                         shared_len=shared_len)
-    return _project(o.reshape(*rows, -1), w_o, projected)
+    return _project(o.flatten(-2), w_o, projected)
 
 
 def _project(o, layer, projected):
