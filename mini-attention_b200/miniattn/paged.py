@@ -171,6 +171,8 @@ def paged_append(
             raise RuntimeError("k and v must have the same shape")
         if k.shape[-2] != k_cache.shape[2]:
             raise RuntimeError("k and the cache must agree in heads")
+        if k.shape[-2] == 0:
+            raise RuntimeError("the number of KV heads must be positive")
         if q is None and q_out is not None:
             raise RuntimeError("q_out without q")
         if q is not None:

@@ -1,4 +1,4 @@
-"""Steps of a serving loop without tokens."""
+"""Calls of the serving operators without tokens or heads."""
 import pytest
 import torch
 
@@ -24,3 +24,12 @@ def test_module_step_without_tokens(kind, ragged):
         assert m.forward_paged(x, *caches, table, lens, cu_q=cu, rope=rope).shape == x.shape
     assert all(bool((c == 1).all()) for c in caches)
     miniattn.check_device_status(DEV)
+
+
+def test_append_without_kv_heads():
+    """Nothing would fill the rotated queries."""
+    q = torch.ones((1, 1, 4, 64), dtype=BF16, device=DEV)
+    none, cache = q[:, :, :0], torch.ones((4, 16, 0, 64), dtype=BF16, device=DEV)
+    table, lens = torch.zeros((1, 2), dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="KV heads"):
+        miniattn.paged_append(none, none, cache, cache, table, lens, q=q)
