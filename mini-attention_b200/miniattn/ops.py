@@ -69,13 +69,15 @@ def check_device_status(device: Union[torch.device, str, None] = None) -> None:
                "device status")
 
 
-def _scratch_for(device: torch.device, stream: int, nbytes: int, *together) -> torch.Tensor:
+def _scratch_for(device: torch.device, stream: int, nbytes: int, together: bool = False) -> torch.Tensor:
     """Scratch of a balanced launch: one buffer per (device, stream), zeroed when created (the
     kernels leave the arrival counters at its start zero again), grown on demand.  A call that is being
     captured gets one of the graph's own memory, since the graph may be replayed on any stream: one buffer
     for all calls that one capture makes on a stream, its counters cleared by the graph before the first.
-    `together` tells buffers of one stream apart (:func:`_launch_together`)."""
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream, *together)
+    `together`: the stream's other buffer (:func:`_launch_together`)."""
+    key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+    if together:
+        key += (together,)
     if torch.cuda.is_current_stream_capturing():
         capture = C.c_uint64(0)
         _lib.check(_lib.lib.miniattn_stream_capture_id(stream, C.byref(capture)), "miniattn_stream_capture_id")
@@ -415,8 +417,8 @@ def _launch_cache(block: bytes, need: int, device: torch.device, several: bool) 
         _lib.check(rc, "miniattn_fwd_cache")
 
 
-def _launch_cache_on(block: bytes, need: int, device: torch.device, stream: int, *together) -> int:
-    scratch = _scratch_for(device, stream, need, *together)
+def _launch_cache_on(block: bytes, need: int, device: torch.device, stream: int, together: bool = False) -> int:
+    scratch = _scratch_for(device, stream, need, together)
     return _lib.lib.miniattn_fwd_cache(block, scratch.data_ptr(), scratch.numel(), stream)
 
 
@@ -429,7 +431,7 @@ def _launch_together(block: bytes, need: int, device: torch.device, stream: int)
     if lock is None:
         lock = _together_locks.setdefault(key, threading.RLock())
     with lock:
-        return _launch_cache_on(block, need, device, stream, "together")
+        return _launch_cache_on(block, need, device, stream, True)
 
 
 # cudaStream_t of torch's current stream on a device without building a Stream object, and the current device
