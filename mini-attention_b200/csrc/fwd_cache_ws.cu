@@ -543,8 +543,9 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         mbar_wait(bar(L::kBarODone + 2 * t + 1), (n_tiles - 1) & 1, wc, kErrWaitO);
         tc_fence_after();
       }
-      // a row that saw no key keeps -inf; its hidden scores left 2^-126 terms in l_run (the polynomial holds its argument)
-      if (m_cur == -INFINITY) l_run = 0.f;
+      // A row that saw no key keeps -inf; its hidden scores left 2^-126 terms in l_run (the polynomial holds its argument).  So
+      // does a row that saw a NaN and in its last half nothing, whose sum stays the NaN it is.
+      if (m_cur == -INFINITY && l_run == l_run) l_run = 0.f;
       auto chunk = [&](int q, uint32_t (&o)[32]) {  // 32 columns of this row's accumulator
         if (n_tiles > 0) {
           tmem_ld32(tO + q * 32, o);

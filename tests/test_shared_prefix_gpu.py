@@ -102,3 +102,23 @@ def test_no_length_in_range():
     _call(p, rows, False)
     with pytest.raises(RuntimeError, match="outside its tensors"):
         miniattn.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("shared", [1056, 1120])   # the last 128 keys' second half is empty, or partly there
+@pytest.mark.parametrize("at", [-1, -40, 500])
+def test_a_key_of_the_prefix_that_is_nan(at, shared):
+    """Every row that sees it is NaN, for the query heads of that KV head; sequences that end before it are not."""
+    lens = [0, 300] + [shared + 1 + i for i in range(B - 2)]
+    p = Paged(lens, [1] * B, HKV, D, BF16, 16, shared=shared, seed=56)
+    rows = list(torch.randn((B, 1, HQ, D), generator=torch.Generator().manual_seed(57)).to(BF16))
+    key = at % shared
+    p.k_cache[int(p.table[5, key // 16]), key % 16, 3] = float("nan")
+    outs, lses = _call(p, rows, False, shared)
+    heads = torch.zeros(HQ, dtype=torch.bool, device=DEV)
+    heads[12:16] = True
+    for b, (o, t, z, tz) in enumerate(zip(*p.expected(rows))):
+        nan = heads & (lens[b] > key)
+        assert torch.equal(outs[b][0].isnan(), nan[:, None].expand(HQ, D)) and torch.equal(lses[b][:, 0].isnan(), nan)
+        check(outs[b][:, ~nan], o[:, ~nan], t[:, ~nan], f"sequence {b}")
+        check(lses[b][~nan], z[~nan], tz[~nan], f"lse of sequence {b}")
+    miniattn.check_device_status(DEV)
