@@ -155,13 +155,18 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
   };
   CacheSeq s{};
   int pairs, tiles, most = 0x7fffffff;  // tiles of a piece
-  if (a.cut > 0 || x == 0) {
+  // Sequences out of range are reported by the first CTA for all, since those left without rows are nobody's item.  Here and not
+  // in the pass below: kept there, `bad` took mixed chunks of 342 us to 348; 40 short sequences gained 0.2 us of 18.9.
+  if (x == 0 && a.status != nullptr) {
+    bool bad = false;
+    for (int b = lane; b < a.B; b += 32) bad |= cache_seq(a, a.cu_q[b], a.cu_q[b + 1], a.seq_lens[b]).bad;
+    if (bad) atomicOr(a.status, kErrCache);
+  }
+  if (a.cut > 0) {
     long long total = 0, items = 0, apart = 0;
     int longest = 0;
-    bool bad = false;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       look(b0 + lane, &s, &pairs, &tiles);
-      bad |= s.bad;
       total += static_cast<long long>(pairs) * tiles;
       items += pairs;
       if (pairs > 0) {
@@ -169,26 +174,22 @@ __device__ __forceinline__ bool ragged_item(const CacheArgs& a, int x, WsItem* i
         longest = max(longest, tiles);
       }
     }
-    // The first CTA reports for all sequences: those that rows out of range leave without any are nobody's item.
-    if (bad && x == 0 && a.status != nullptr) atomicOr(a.status, kErrCache);
-    if (a.cut > 0) {
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, d);
-        items += __shfl_xor_sync(0xffffffffu, items, d);
-        apart += __shfl_xor_sync(0xffffffffu, apart, d);
-      }
-      longest = __reduce_max_sync(0xffffffffu, longest);
-      const long long even = (total * a.groups + a.cut - 1) / a.cut;
-      // Rows that overlap, which only row numbers that fall give, may be more than the launch has CTAs for: a piece without one
-      // would leave its item's counter standing, so nothing is cut then.
-      if (items * a.groups + a.cut <= gridDim.x) most = clamp_to(even, 2 * a.min_tiles, 0x7fffffff);
-      // 2 x 128 tokens against 1600 keys, 32/8 heads of 128: 21.6 us, 26.2 in pieces of pairs; 300 against 2040, 8/2 heads 24.0
-      // and 27.0.  Not where most pairs are single tiles as it is (3 x 100 tokens, 12 heads: 24.9, 23.1 in pieces).
-      if (2 * apart * a.groups <= a.cut && 2 * apart >= 3 * items && longest <= max(most, 4 * a.min_tiles)) {
-        span = a.tpt;
-        most = 0x7fffffff;
-      }
+    for (int d = 16; d > 0; d >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, d);
+      items += __shfl_xor_sync(0xffffffffu, items, d);
+      apart += __shfl_xor_sync(0xffffffffu, apart, d);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    const long long even = (total * a.groups + a.cut - 1) / a.cut;
+    // Rows that overlap, which only row numbers that fall give, may be more than the launch has CTAs for: a piece without one
+    // would leave its item's counter standing, so nothing is cut then.
+    if (items * a.groups + a.cut <= gridDim.x) most = clamp_to(even, 2 * a.min_tiles, 0x7fffffff);
+    // 2 x 128 tokens against 1600 keys, 32/8 heads of 128: 21.6 us, 26.2 in pieces of pairs; 300 against 2040, 8/2 heads 24.0
+    // and 27.0.  Not where most pairs are single tiles as it is (3 x 100 tokens, 12 heads: 24.9, 23.1 in pieces).
+    if (2 * apart * a.groups <= a.cut && 2 * apart >= 3 * items && longest <= max(most, 4 * a.min_tiles)) {
+      span = a.tpt;
+      most = 0x7fffffff;
     }
   }
   long long before = 0;  // pieces of the sequences before
