@@ -313,10 +313,12 @@ int miniattn_linear(const MiniAttnLinearParams* p, void* stream);
  * behind the last one's are left as they are.  Null: Nq rows each.
  *
  * shared_len: the first shared_len tokens of all sequences are the same, the rows of the block table begin with the same
- * pages; their keys are read once for all where that is quicker.  A multiple of page_size; not with a window.
+ * pages.  Where a KV head has at most 32 rows (tokens of a sequence x query heads) and their keys and values would be 100 MB
+ * if every sequence read its own, they are read once for all.  A multiple of page_size; not with a window.
  *
- * A length, row number or page outside the call's tensors sets bit 7 of the status word; nothing outside them is read or
- * written, and the sequence's results are undefined, the others' are not.
+ * A length, row number or page outside the call's tensors sets bit 7 of the status word, also where the sequence has no rows;
+ * nothing outside them is read or written, and the sequence's results are undefined, the others' are not.  Row numbers that fall
+ * leave the whole call's results undefined, and so does a page of the shared prefix that lies outside.
  *
  * Lengths, rows and pages are read on the device: a captured launch serves every length the block table has room for.
  */
@@ -351,10 +353,11 @@ typedef struct MiniAttnCacheParams {
   float   softmax_scale;  /* <= 0 selects 1/sqrt(D)                                    */
 } MiniAttnCacheParams;
 
-/* scratch: as for miniattn_fwd_balanced, miniattn_fwd_cache_scratch_bytes(p) bytes; not optional.  With shared_len
- * the call may make several launches that hand results on in it: between them no other thread may enqueue a call that uses the same
- * scratch, so threads that share a stream need a scratch each, or a lock around the call.  That size depends on the
- * sizes in `p` alone; pointers are compared with null and not read. */
+/* scratch: as for miniattn_fwd_balanced, miniattn_fwd_cache_scratch_bytes(p) bytes; not optional.  That size depends on the
+ * sizes and, with shared_len, on the strides of q in `p`; pointers are compared with null and not read.
+ *
+ * With shared_len the call may make several launches that hand results on in the scratch.  Between them no other thread may
+ * enqueue a call that uses the same scratch: threads that share a stream need a scratch each, or a lock around the call. */
 int miniattn_fwd_cache(const MiniAttnCacheParams* p, void* scratch, size_t scratch_bytes, void* stream);
 int64_t miniattn_fwd_cache_scratch_bytes(const MiniAttnCacheParams* p);
 
@@ -365,8 +368,9 @@ int64_t miniattn_fwd_cache_scratch_bytes(const MiniAttnCacheParams* p);
  * rope: [rope_rows, rot] fp32, the cosines of the rot / 2 angles of each position and then their sines; null: nothing is
  * rotated.  Pairs are elements (i, i + rot / 2), with `interleaved` (2i, 2i + 1); elements from rot on stay as they are.
  * Tokens before position 0 (the front of a padded sequence) are left out, their rows of q copied.  A position past the block
- * table or the rotation table, a page outside the cache, rows outside the call's or that fall, or a negative length set bit 7
- * of the status word; the token is left out.  Two tokens of one call must not go to the same place.
+ * table or the rotation table, a page outside the cache, rows outside the call's or that fall, or a length that is negative or
+ * past the block table set bit 7 of the status word; the token is left out (where rows fall, perhaps tokens of other sequences).
+ * Two tokens of one call must not go to the same place.
  */
 typedef struct MiniAttnAppendParams {
   const void* k;

@@ -1054,7 +1054,8 @@ struct CachePlan {
 
 constexpr int kMinPieceTiles = 4;      // 128-key tiles of a piece
 constexpr int kMinPrefixTiles = 2;     // of a shared prefix's, whose pieces a launch of its own adds up
-constexpr long long kMaxPieces = 480;  // of all items together: 64 MB of scratch at D = 128
+// Pieces of all items together.  Scratch at D = 128: 64 MB; ragged calls have 2 x SMs more, 39 MB at least and 103 at most.
+constexpr long long kMaxPieces = 480;
 
 // Pieces that items of at most `tiles` tiles are cut into where all are alike.  A CTA takes its tiles and about 4 steps of a
 // tile's time beside them; a piece takes 2 more to leave its result, the last 0.8 for each piece it folds.
@@ -1093,7 +1094,8 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
     // What all sequences would read of it without: the two launches more and the pieces between them cost about as much as
     // 100 MB of it.  With and without, 32/8 heads of 128: 16 x 1024 tokens (67 MB) 17.1 / 15.9 us, 64 x 512 (134) 27.1 / 26.1,
     // 32 x 1024 (134) 18.2 / 22.2, 16 x 4096 (268) 18.9 / 29.5, 64 x 2048 (537) 29.7 / 53.7; 8/2 heads of 64: 64 x 2048 (67)
-    // 16.8 / 16.8.
+    // 16.8 / 16.8.  One or two sequences, which save nothing or half, lose by it: 1 x 32768 (134) 42.9 / 37.0, 2 x 16384 (134)
+    // 24.4 / 23.7, 2 x 32768 (268) 42.1 / 39.0; 4 x 8192 (134) 19.9 / 20.4, 4 x 32768 (537) 41.6 / 52.6.
     const long long row_blocks = (rows + 16 * c.rg - 1) / (16 * c.rg);
     const double read = 4.0 * p->B * p->Hkv * row_blocks * p->shared_len * kernel_head_dim(p->D);
     if (read >= 1e8 && p->n_pages > 0 && stacked && pairs * c.groups <= kMaxPieces) {
@@ -1112,14 +1114,18 @@ CachePlan cache_plan(const MiniAttnCacheParams* p, int sms) {
   c.ctas = c.pair_items = static_cast<int>(std::min<long long>(items, 0x7fffffff));
   c.parts = 1;
   if (ragged) {
-    if (items <= kMaxPieces) {  // many more come out even without
+    // Above that nothing is cut: 60 requests of 500 to 8000 keys that decode beside a chunk of 2048 tokens against 4000, 32/8 heads
+    // (744 items), take 351 us, the requests alone 164 in fwd_cache.cu and the chunk alone 152.
+    if (items <= kMaxPieces) {
       c.cut = 2 * sms;
       c.ctas += c.cut;
       c.part_rows = static_cast<size_t>(c.ctas) * 2 * ma::kTileM;
     }
     return c;
   }
-  const auto seen_by = [&](long long tokens) {  // in tiles, at most
+  // In tiles, at most: lengths are not known here, so a block table that is wider than its sequences are long counts as keys (the
+  // chunk of 128 tokens against 1024 keys below: 14.5 us with a table for 1152 tokens, 20.3 and cut with one for 2048 or more).
+  const auto seen_by = [&](long long tokens) {
     return tiles_of(p->window > 0 ? std::min(room, static_cast<long long>(p->window) + p->sinks + tokens + 256) : room);
   };
   float least = 0.f;

@@ -15,8 +15,9 @@
 // A CTA whose range cuts an item leaves its piece (un-normalised O, m, l) in scratch and counts itself in; the one that
 // counts in last folds the pieces.  Behind a shared prefix the rows are left un-normalised for the launch that adds its pieces.
 //
-// Bound: HBM where the contexts are long: 16 requests of 1001 to 16001 keys, 32/8 heads of 128, pages of 16 tokens 67 us = 5.6
-// TB/s, 0.86 of the measured copy rate; 32 with a window of 4096 87 us = 6.0 TB/s.  Short calls are bound by their chain of
+// Bound: HBM where the contexts are long: 16 requests of 1001 to 16001 keys, 32/8 heads of 128, pages of 16 tokens 67.5 us = 5.6
+// TB/s, 0.85 of the measured copy rate; 32 with a window of 4096 90 us = 5.8 TB/s, 0.89.  The registers of two CTAs an SM: 32
+// bytes spill at D = 128 with one row group.  Short calls are bound by their chain of
 // loads: lengths (0.7 us), the walk to the CTA's range (0.8), block table and first tile (1.2), half a microsecond a tile, 0.5
 // to leave a piece and 3 to fold: 4 requests of 100 to 1000 keys, 12 heads of 64 9 us (pieces of 4 tiles; of 6, 8 and 12: 9.5,
 // 10.1, 11.9, with an earlier fold).

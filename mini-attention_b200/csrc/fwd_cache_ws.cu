@@ -14,7 +14,7 @@
 // Tiles at the ends hold keys that no row of the sequence sees and that may be anything.  Their scores are replaced; their
 // rows of V are cleared in shared memory by warp 11, which hands such a tile over itself instead of leaving that to the copy.
 //
-// Bound: tensor pipe and power where items are long (16384 tokens, 32/8 heads of 128, window 4096, 4 sinks 860 us = 1.1 PFLOP/s;
+// Bound: tensor pipe and power where items are long (16384 tokens, 32/8 heads of 128, window 4096, 4 sinks 878 us = 1.1 PFLOP/s;
 // 1.7 us a 128-key step of a CTA at the power cap).  Short windows are bound by a CTA's ends and by the tiles that only some of
 // its 256 rows see: 4 x 1024 tokens, 12 heads of 64, window 256 20.6 us, 3 us of an item's 12 outside its steps.
 //
@@ -526,6 +526,7 @@ fwd_cache_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                   p1 = ex2(x1);
                 }
                 psum = add_f32x2(psum, pack_f32x2(p0, p1));
+                // P in 16 bits for the second product: off by half a step of the type for each weight
                 pk[q * 16 + (i >> 1)] = pack2<BF16>(p0, p1);
               }
             unpack_f32x2(psum, psum0, psum1);

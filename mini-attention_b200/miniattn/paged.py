@@ -14,9 +14,10 @@ later steps as well.  The conventions both share:
 * New tokens come as (B, n, heads, D), or ragged as (rows, heads, D) with ``cu_q``, (B + 1,) int32: the rows of sequence b are
   ``cu_q[b]`` to ``cu_q[b + 1] - 1``.  Rows before the first sequence's and behind the last one's are left as they are.
 
-A length, row, page or position outside these tensors is found on the device: it sets a bit that
-:func:`miniattn.check_device_status` turns into an error, nothing outside them is read or written, and that sequence's results
-are undefined.  The tensors must not change while a call runs.
+A length, row, page or position outside these tensors is found on the device, also in a sequence that has no rows: it sets a bit
+that :func:`miniattn.check_device_status` turns into an error, nothing outside them is read or written, and that sequence's
+results are undefined.  Row numbers that fall leave those of the whole call undefined, and so does a page outside the cache among
+those of a shared prefix.  The tensors must not change while a call runs.
 """
 from __future__ import annotations
 
@@ -151,8 +152,9 @@ def paged_append(
     rotated by their positions on the way, and so is ``q``, the queries of the same tokens, which come back in ``q_out``
     (a new tensor by default; ``q`` itself is fine, any other overlap is not).  Pairs are elements (i, i + width / 2) of a
     head, neighbours (2 i, 2 i + 1) with ``interleaved``.  Tokens at negative positions (the front of a padded sequence,
-    ``seq_lens[b] < n``) are left out and their queries copied.  Two tokens of one call must not go to the same place of the
-    cache, which a block table that gives a page to one writing sequence at a time ensures.
+    ``seq_lens[b] < n``) are left out and their queries copied; so are tokens whose position or page is out of range.  Two
+    tokens of one call must not go to the same place of the cache, which a block table that gives a page to one writing
+    sequence at a time ensures.
 
     Returns the rotated queries, or None without ``q``.
     """
@@ -247,10 +249,14 @@ def paged_attention(
 
     ``max_q``, with ``cu_q``: the most rows that one sequence has.  It picks the kernel and nothing else; without it the rows
     of ``q`` are taken for it.  ``shared_len``: the first ``shared_len`` tokens (whole pages) are the same for all sequences,
-    the rows of the block table begin with the same pages; they are read once for the whole batch where that is quicker.
+    the rows of the block table begin with the same pages.  Decode and drafts (up to 32 rows of a KV head: tokens of a sequence
+    x query heads that share it) read them once for the whole batch where 100 MB would be read otherwise; other calls, and shorter
+    prefixes, are read sequence by sequence.
 
     Returns ``out`` or ``(out, lse)``, lse fp32, the natural logarithm of the softmax denominators: (B, Hq, n), or (Hq, rows)
-    with ``cu_q``.  A NaN or infinity among the values of a key that any row of a sequence sees may show in others of its rows.
+    with ``cu_q``.  A key that is NaN makes the rows that see it NaN, and no others.  A NaN or infinity among the *values* of a key
+    that any row of a sequence sees may show in others of its rows, among those of a shared prefix in the rows of every
+    sequence that holds some of its tokens.
     """
     if max_q is not None and type(max_q) is not int:
         max_q = _as_int("max_q", max_q)

@@ -122,3 +122,13 @@ def test_a_key_of_the_prefix_that_is_nan(at, shared):
         check(outs[b][:, ~nan], o[:, ~nan], t[:, ~nan], f"sequence {b}")
         check(lses[b][~nan], z[~nan], tz[~nan], f"lse of sequence {b}")
     miniattn.check_device_status(DEV)
+
+
+def test_row_numbers_that_leave_the_queries():
+    """Reported; the sequences before are right, rows of the last one that are there are left out or undefined."""
+    p, rows = _batch([SHARED + 5 + 11 * i for i in range(B)], [1] * B, seed=58)
+    p.cu_q[B] = B + 3
+    outs, lses = _call(p, rows, True)
+    with pytest.raises(RuntimeError, match="outside its tensors"):
+        miniattn.check_device_status(DEV)
+    _right(p, rows, outs, lses, but=(B - 1,))
