@@ -10,6 +10,7 @@ device memory and streams only; the arithmetic runs in libminiattn.so.
 from __future__ import annotations
 
 import ctypes as C
+import numbers
 import operator
 import struct
 import threading
@@ -334,7 +335,7 @@ def _as_int(name: str, x) -> int:
         return operator.index(x)
     except TypeError:
         pass
-    if isinstance(x, float) and x.is_integer():
+    if isinstance(x, numbers.Real) and float(x).is_integer():
         return int(x)
     raise RuntimeError(f"{name} must be a whole number, got {x!r}")
 

@@ -1,4 +1,5 @@
 """Numbers of a call that come as 0-dim tensors: a call goes by what they hold then.  What is no whole number is refused."""
+import numpy as np
 import pytest
 import torch
 
@@ -80,4 +81,8 @@ def test_what_is_no_whole_number(name, value):
 
 def test_whole_numbers_of_other_types():
     from miniattn.ops import _as_int
-    assert [_as_int("n", x) for x in (3, True, 3.0, torch.tensor(3), torch.tensor(3.0), torch.tensor([3]))] == [3, 1, 3, 3, 3, 3]
+    others = (3, True, 3.0, np.int64(3), np.float32(3), torch.tensor(3), torch.tensor(3.0), torch.tensor([3]))
+    assert [_as_int("n", x) for x in others] == [3, 1, 3, 3, 3, 3, 3, 3]
+    for x in (float("nan"), float("inf"), None, 3j):
+        with pytest.raises(RuntimeError, match="whole number"):
+            _as_int("n", x)
