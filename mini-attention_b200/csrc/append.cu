@@ -50,8 +50,8 @@ __device__ __forceinline__ int sequence_of(const AppendArgs& a, int t) {
 // kWarps warps take a row together: one where the rows fill the GPU (the three loads of a row's lookups, which wait for one
 // another, are then hidden by the other rows of the SM), eight where they do not.  7 prompts of 7261 tokens in all, 32/8 heads of
 // 128: 36.7 us = 5.0 TB/s, 0.76 of the copy rate (49 with a CTA to a row); 4 x 8192 tokens, 16/4 heads of 64: 39.9 us = 5.1
-// TB/s (89).  Two heads of a lane in flight and three CTAs an SM (4 to 16 bytes spill): 1 and 4 took 37.6 and 40.6 us, 4 and 2 34.5 and 41.7, 3 and 3
-// 39.6 and 44.2.  A step of decode (32 rows) takes 2.5 us, a launch and those three loads.
+// TB/s (89).  Two heads of a lane in flight and three CTAs an SM (4 to 16 bytes spill): 1 and 4 took 37.6 and 40.6 us, 4 and 2
+// 34.5 and 41.7, 3 and 3 39.6 and 44.2.  A step of decode (32 rows) takes 2.5 us, a launch and those three loads.
 template <bool BF16, int kWarps>
 __global__ void __launch_bounds__(kThreads, 3)
 append_kernel(const AppendArgs a) {
